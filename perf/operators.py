@@ -137,7 +137,7 @@ def work(case):
 def _quantised(x, kv_heads):
     """[slots, row] -> E4M3 codes [slots, row] and scales [kv_heads, slots]: how a cache was filled."""
     h = x.view(x.shape[0], kv_heads, -1)
-    scale = (h.abs().amax(-1) / E4M3_MAX).clamp_min(LEAST_SCALE)
+    scale = (h.abs().amax(-1) / torch.tensor(E4M3_MAX, device=x.device)).clamp_min(LEAST_SCALE)
     return (h / scale[..., None]).to(torch.float8_e4m3fn).reshape(x.shape), scale.t().contiguous()
 
 

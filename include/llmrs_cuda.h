@@ -44,7 +44,8 @@ enum llmrs_dtype {
     LLMRS_Q4K = 12,
     LLMRS_Q6K = 14,
     LLMRS_I32 = 26,     /* index buffers (positions, slot mapping, page tables), as upload_u32 makes them */
-    LLMRS_BF16 = 30
+    LLMRS_BF16 = 30,
+    LLMRS_E4M3 = 256    /* codes of the 8-bit KV cache (scatter_kv_quant ... attention_quant); not a GGUF type */
 };
 
 /* Device layout of a buffer's bytes. */
@@ -272,6 +273,92 @@ int llmrs_cuda_matmul_gate_up(llmrs_ctx *ctx, llmrs_buf *out, const llmrs_buf *w
 int llmrs_cuda_embed(llmrs_ctx *ctx, llmrs_buf *out, const llmrs_buf *table, const uint32_t *tokens,
                      uint32_t n_tokens);
 
+/* ---- scaled rotary positions and the 8-bit KV cache -----------------------------------------------
+ * The calls of a layer between the q/k/v projections and wo (src/arch/llama.rs:156-161) for contexts that
+ * are longer than a model was trained on and caches that are larger than memory in 16 bits.  The reference
+ * has neither; each call stands in for the one it is named after.
+ *
+ * Cache: k_pool and v_pool are E4M3 buffers [kv_dim, slots] (kv_dim = n_kv_heads * head_dim), addressed like
+ * the pools of scatter_kv; k_scales and v_scales F32 buffers [slots, n_kv_heads], all created by alloc, wrap
+ * or (codes saved earlier) upload_tensor.  Element d of head h of a slot is code * scale, where the write
+ * calls set   scale = max(largest magnitude of the head's values / 448, 2^-126)  in float32 and
+ * code = E4M3(value / scale), rounded to nearest even: half a step of E4M3, 2^-4 of a value, at most, or 2^-10
+ * scale of one below 2^-6 scale.  A head with a value that is not finite gets the scale NaN and codes 0: rows of
+ * attention that see the position come out NaN, others do not notice.  The pools need no initialisation; codes
+ * other than those the write calls make must be finite (not 0x7F / 0xFF).
+ *
+ * Index buffers are device memory: what they name is checked by the kernels.  A slot, page or length beyond
+ * the pool or the page table is neither read nor written, and the next llmrs_cuda_sync / read_f32 returns
+ * LLMRS_ERR_ARG.  All buffers must live on the context's device, and outputs must not overlap inputs except
+ * where a call says so. */
+
+/* How rope frequencies are stretched for a context of more positions than the model was trained on. */
+enum llmrs_rope_scaling_kind {
+    LLMRS_ROPE_NONE = 0,
+    LLMRS_ROPE_LINEAR = 1,      /* every frequency / factor */
+    LLMRS_ROPE_WAVELENGTH = 2,  /* turns over the original context t = f * original_context / 2 pi: f / factor where
+                                   t < low, f where t > high, between them the mix with weight (t - low) / (high - low) */
+    LLMRS_ROPE_YARN = 3         /* f up to the index that makes `high` turns over the original context (rounded
+                                   down, at least 0), f / factor from the one that makes `low` (rounded up, at most
+                                   rotary_dim - 1), a linear mix between them; magnitude 1 + 0.1 ln(factor) */
+};
+typedef struct llmrs_rope_scaling {
+    uint32_t kind;              /* llmrs_rope_scaling_kind */
+    uint32_t original_context;  /* positions the model was trained on (WAVELENGTH, YARN) */
+    float factor;               /* >= 1 */
+    float low, high;            /* turns: WAVELENGTH usually 1 and 4, YARN 1 and 32 */
+} llmrs_rope_scaling;
+
+/* The frequency table of rope_scaled and rope_scatter_kv_quant: inv_freq[i], i < rotary_dim / 2, from
+ * f = rope_theta^(-2 i / rotary_dim), stretched by `scaling` (NULL: not), then divided by factors[i] where a
+ * file brings such a list (rope_freqs.weight; NULL: none); computed in double and rounded once.  *magnitude
+ * is what the rotated values are to be multiplied by.  Host memory, no context and no GPU; the message of a
+ * failure is llmrs_cuda_last_error(NULL).  rotary_dim even, 2 .. 256. */
+int llmrs_cuda_rope_frequencies(uint32_t rotary_dim, float rope_theta, const llmrs_rope_scaling *scaling,
+                                const float *factors, float *inv_freq, float *magnitude);
+
+/* Rotary positions from a table: the first rotary_dim = 2 * inv_freq.dim0 values of each head of q and k are
+ * rotated by position * inv_freq[i] and multiplied by `magnitude`, the others copied.  split_half = 0 rotates
+ * pairs (2i, 2i+1), 1 pairs (i, i + rotary_dim/2).  The angle is reduced in float64, so that position 131072
+ * is as exact as position 1.  q and k [heads * head_dim, tokens], F32 or BF16, all four of one type;
+ * q_out may be q itself and k_out k itself.  head_dim even, at most 256.  positions: I32, read as unsigned. */
+int llmrs_cuda_rope_scaled(llmrs_ctx *ctx, llmrs_buf *q_out, llmrs_buf *k_out, const llmrs_buf *q, const llmrs_buf *k,
+                           const llmrs_buf *positions, const llmrs_buf *inv_freq, uint32_t head_dim, float magnitude,
+                           uint32_t split_half);
+
+/* scatter_kv into an 8-bit pool: row t of src [kv_dim, >= num_tokens] (F32 or BF16) is quantised, a scale a
+ * head, into slot slot_mapping[t].  kv_dim and the slots are the pool's, n_kv_heads the scales' dim1 and
+ * head_dim = kv_dim / n_kv_heads, even and at most 256.  Slot 0xFFFFFFFF marks a padding token: nothing is
+ * written for it.  The other slots of a call must differ from one another. */
+int llmrs_cuda_scatter_kv_quant(llmrs_ctx *ctx, llmrs_buf *pool, llmrs_buf *scales, const llmrs_buf *src,
+                                const llmrs_buf *slot_mapping, uint32_t num_tokens);
+
+/* rope_scaled of q (into q_out, which may be q) and k, and scatter_kv_quant of the rotated k and of v, as one
+ * call and one launch.  k and v are only read; the rotated k is quantised from float32 without a rounding to
+ * its own type in between.  q_out, q, k and v of one type (F32 or BF16). */
+int llmrs_cuda_rope_scatter_kv_quant(llmrs_ctx *ctx, llmrs_buf *q_out, const llmrs_buf *q, const llmrs_buf *k,
+                                     const llmrs_buf *v, const llmrs_buf *positions, const llmrs_buf *inv_freq,
+                                     uint32_t head_dim, float magnitude, uint32_t split_half, llmrs_buf *k_pool,
+                                     llmrs_buf *k_scales, llmrs_buf *v_pool, llmrs_buf *v_scales,
+                                     const llmrs_buf *slot_mapping);
+
+/* gather from an 8-bit pool: column c of out ([kv_dim, >= num_indices], F32 or BF16) = slot indices[c] read
+ * back, code * scale in float32 and one rounding.  A column whose index is beyond the pool keeps what it held. */
+int llmrs_cuda_gather_quant(llmrs_ctx *ctx, llmrs_buf *out, const llmrs_buf *pool, const llmrs_buf *scales,
+                            const llmrs_buf *indices, uint32_t num_indices);
+
+/* llmrs_cuda_attention over an 8-bit cache: the same paged, variable-length, grouped-query, causal attention,
+ * its arguments of the same meaning.  q and out F32 or BF16, of one type; n_heads any multiple of n_kv_heads,
+ * head_dim a multiple of 32, at most 256.  Positions on a page beyond the pool count as unseen; a query token that
+ * sees no position (its request is shorter than its query tokens) yields zeros; tokens behind the last
+ * request keep what out held.  Like llmrs_cuda_attention it uses a workspace of the context, so graphs captured
+ * from one context must not run at the same time. */
+int llmrs_cuda_attention_quant(llmrs_ctx *ctx, llmrs_buf *out, const llmrs_buf *q, const llmrs_buf *k_pool,
+                               const llmrs_buf *k_scales, const llmrs_buf *v_pool, const llmrs_buf *v_scales,
+                               const llmrs_buf *block_table, const llmrs_buf *query_starts, const llmrs_buf *seq_lens,
+                               uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim, uint32_t block_size,
+                               uint32_t max_blocks_per_seq);
+
 /* Multi-GPU decode matmul: this rank's rows of an N-sharded weight, with the all-gather of the
  * output slices fused into the kernel.  The reference is single-GPU and has no counterpart; the
  * sharding follows from every output row reading only its own weight row (shaders/ops.metal:249-289).
@@ -342,7 +429,7 @@ size_t llmrs_cuda_perf_table(llmrs_ctx *ctx, char *buf, size_t cap);
 /* Number of kernels this library has launched on the context since creation. */
 int llmrs_cuda_launch_count(llmrs_ctx *ctx, uint64_t *count);
 
-/* Message of the last failure on `ctx` (or of the last failed create when ctx is NULL). */
+/* Message of the last failure on `ctx` (or of the last failed create or rope_frequencies when ctx is NULL). */
 const char *llmrs_cuda_last_error(llmrs_ctx *ctx);
 
 /* ---- GGUF files: the on-disk step in front of upload_tensor --------------------------------------

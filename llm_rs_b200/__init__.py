@@ -3,4 +3,5 @@
 `CudaBackend` mirrors the reference's `Backend` trait for the matmul path and calls the
 hand-written CUDA kernels through the C ABI in include/llmrs_cuda.h.
 """
-from .backend import BackendError, CudaBackend, CudaBuffer, DType, TensorView, load_library  # noqa: F401
+from .backend import (BackendError, CudaBackend, CudaBuffer, DType, RopeScaling, TensorView, load_library,  # noqa: F401
+                      rope_frequencies)

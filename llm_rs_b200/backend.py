@@ -34,12 +34,13 @@ class DType(enum.IntEnum):
     Q6K = 14
     I32 = 26
     BF16 = 30
+    E4M3 = 256        # codes of the 8-bit KV cache; not a GGUF type
 
     def block_elems(self) -> int:                     # src/tensor/mod.rs:37-50
         return 256 if self in (DType.Q4K, DType.Q6K) else 32 if self in (DType.Q4_0, DType.Q8_0) else 1
 
     def block_size_bytes(self) -> int:                # src/tensor/mod.rs:52-86
-        return {DType.F32: 4, DType.I32: 4, DType.BF16: 2, DType.F16: 2, DType.Q4_0: 18, DType.Q8_0: 34,
+        return {DType.F32: 4, DType.I32: 4, DType.BF16: 2, DType.F16: 2, DType.E4M3: 1, DType.Q4_0: 18, DType.Q8_0: 34,
                 DType.Q4K: 144, DType.Q6K: 210}[self]
 
     def storage_size(self, n_elements: int) -> int:   # src/tensor/mod.rs:89-93
@@ -83,6 +84,12 @@ class _Buf(C.Structure):
                 ("dim1", C.c_uint32), ("layout", C.c_uint32), ("owned", C.c_uint32), ("device", C.c_uint32)]
 
 
+class _RopeScaling(C.Structure):
+    """llmrs_rope_scaling."""
+    _fields_ = [("kind", C.c_uint32), ("original_context", C.c_uint32), ("factor", C.c_float), ("low", C.c_float),
+                ("high", C.c_float)]
+
+
 # Every symbol include/llmrs_cuda.h declares: (restype, argtypes).
 _VP, _U64P = C.c_void_p, C.POINTER(C.c_uint64)
 _BUFP = C.POINTER(_Buf)
@@ -107,6 +114,13 @@ ABI = {
     "llmrs_cuda_scatter_kv": (C.c_int, [_VP, _BUFP, _BUFP, _BUFP, C.c_uint32, C.c_uint32]),
     "llmrs_cuda_gather": (C.c_int, [_VP, _BUFP, _BUFP, _BUFP, C.c_uint32]),
     "llmrs_cuda_attention": (C.c_int, [_VP] + [_BUFP] * 7 + [C.c_uint32] * 5),
+    "llmrs_cuda_rope_frequencies": (C.c_int, [C.c_uint32, C.c_float, C.POINTER(_RopeScaling), C.POINTER(C.c_float),
+                                              C.POINTER(C.c_float), C.POINTER(C.c_float)]),
+    "llmrs_cuda_rope_scaled": (C.c_int, [_VP] + [_BUFP] * 6 + [C.c_uint32, C.c_float, C.c_uint32]),
+    "llmrs_cuda_scatter_kv_quant": (C.c_int, [_VP] + [_BUFP] * 4 + [C.c_uint32]),
+    "llmrs_cuda_rope_scatter_kv_quant": (C.c_int, [_VP] + [_BUFP] * 6 + [C.c_uint32, C.c_float, C.c_uint32] + [_BUFP] * 5),
+    "llmrs_cuda_gather_quant": (C.c_int, [_VP] + [_BUFP] * 4 + [C.c_uint32]),
+    "llmrs_cuda_attention_quant": (C.c_int, [_VP] + [_BUFP] * 9 + [C.c_uint32] * 5),
     "llmrs_cuda_rms_norm_matmul": (C.c_int, [_VP, _BUFP, _BUFP, _BUFP, _BUFP, C.c_float]),
     "llmrs_cuda_rms_norm_matmul_gate_up": (C.c_int, [_VP, _BUFP, _BUFP, _BUFP, _BUFP, _BUFP, C.c_float]),
     "llmrs_cuda_rms_norm_matmul_qkv": (C.c_int, [_VP] + [_BUFP] * 8 + [C.c_float]),
@@ -166,12 +180,45 @@ def load_library() -> C.CDLL:
     return _lib
 
 
+class RopeScaling(enum.IntEnum):
+    """How rope frequencies are stretched for long contexts (enum llmrs_rope_scaling_kind)."""
+    NONE = 0
+    LINEAR = 1
+    WAVELENGTH = 2
+    YARN = 3
+
+
+def rope_frequencies(rotary_dim: int, rope_theta: float, kind: RopeScaling = RopeScaling.NONE, factor: float = 1.0,
+                     original_context: int = 0, low: float = 1.0, high: float = 4.0,
+                     factors: Sequence[float] | None = None) -> tuple[np.ndarray, float]:
+    """The frequency table (float32 [rotary_dim / 2]) and the magnitude that rope_scaled and rope_scatter_kv_quant
+    take: rope_theta^(-2 i / rotary_dim), stretched as `kind` says, divided by `factors` (a file's rope_freqs.weight).
+    `low` and `high` are turns over the original context: usually 1 and 4 for WAVELENGTH, 1 and 32 for YARN.  No GPU."""
+    lib = load_library()
+    if rotary_dim < 0 or original_context < 0:
+        raise ValueError(f"rope_frequencies: rotary_dim {rotary_dim}, original_context {original_context}")
+    out = np.empty(max(rotary_dim // 2, 1), dtype=np.float32)
+    mag = C.c_float()
+    fac = None
+    if factors is not None:
+        fac = np.ascontiguousarray(factors, dtype=np.float32).reshape(-1)
+        if fac.size != rotary_dim // 2:
+            raise ValueError(f"rope_frequencies: {fac.size} factors for {rotary_dim // 2} frequencies")
+    fp = C.POINTER(C.c_float)
+    rc = lib.llmrs_cuda_rope_frequencies(rotary_dim, rope_theta, C.byref(_RopeScaling(int(kind), original_context, factor, low, high)),
+                                         None if fac is None else fac.ctypes.data_as(fp), out.ctypes.data_as(fp), C.byref(mag))
+    if rc != 0:
+        raise BackendError(rc, (lib.llmrs_cuda_last_error(None) or b"").decode())
+    return out, float(mag.value)
+
+
 class CudaBuffer:
     """Device buffer + dtype + dims: the counterpart of MetalBuffer (metal/mod.rs:13-34)."""
 
     def __init__(self, backend: "CudaBackend", raw: _Buf, keepalive=None):
         self._backend = backend
         self._raw = raw
+        self._ref = C.byref(raw)
         self._keepalive = keepalive       # e.g. the torch tensor whose memory is wrapped
 
     dtype = property(lambda self: DType(self._raw.dtype))
@@ -369,6 +416,43 @@ class CudaBackend:
                                                    C.byref(v_pool._raw), C.byref(block_table._raw),
                                                    C.byref(query_starts._raw), C.byref(seq_lens._raw), n_heads,
                                                    n_kv_heads, head_dim, block_size, max_blocks_per_seq))
+
+    # -- scaled rotary positions and the 8-bit KV cache (no trait counterpart) --
+    def rope_scaled(self, q_out: CudaBuffer, k_out: CudaBuffer, q: CudaBuffer, k: CudaBuffer, positions: CudaBuffer,
+                    inv_freq: CudaBuffer, head_dim: int, magnitude: float = 1.0, split_half: bool = False) -> None:
+        """Rotates the first 2 * inv_freq.dim0 values of each head of q and k by position * inv_freq[i], times
+        `magnitude` (both from rope_frequencies).  q_out may be q and k_out may be k."""
+        self._check(self._lib.llmrs_cuda_rope_scaled(self._ctx, q_out._ref, k_out._ref, q._ref, k._ref, positions._ref,
+                                                     inv_freq._ref, head_dim, magnitude, 1 if split_half else 0))
+
+    def scatter_kv_quant(self, pool: CudaBuffer, scales: CudaBuffer, src: CudaBuffer, slot_mapping: CudaBuffer,
+                         num_tokens: int) -> None:
+        """scatter_kv into an 8-bit pool: pool E4M3 [kv_dim, slots], scales F32 [slots, n_kv_heads].  Slot 0xFFFFFFFF
+        marks a padding token."""
+        self._check(self._lib.llmrs_cuda_scatter_kv_quant(self._ctx, pool._ref, scales._ref, src._ref, slot_mapping._ref,
+                                                          num_tokens))
+
+    def rope_scatter_kv_quant(self, q_out: CudaBuffer, q: CudaBuffer, k: CudaBuffer, v: CudaBuffer, positions: CudaBuffer,
+                              inv_freq: CudaBuffer, head_dim: int, magnitude: float, k_pool: CudaBuffer, k_scales: CudaBuffer,
+                              v_pool: CudaBuffer, v_scales: CudaBuffer, slot_mapping: CudaBuffer,
+                              split_half: bool = False) -> None:
+        """rope_scaled of q (into q_out, which may be q) and k, then scatter_kv_quant of the rotated k and of v, as one
+        call and one launch; k and v are only read."""
+        self._check(self._lib.llmrs_cuda_rope_scatter_kv_quant(
+            self._ctx, q_out._ref, q._ref, k._ref, v._ref, positions._ref, inv_freq._ref, head_dim, magnitude,
+            1 if split_half else 0, k_pool._ref, k_scales._ref, v_pool._ref, v_scales._ref, slot_mapping._ref))
+
+    def gather_quant(self, out: CudaBuffer, pool: CudaBuffer, scales: CudaBuffer, indices: CudaBuffer, num_indices: int) -> None:
+        """gather from an 8-bit pool: column c of out (F32 or BF16) = slot indices[c] read back."""
+        self._check(self._lib.llmrs_cuda_gather_quant(self._ctx, out._ref, pool._ref, scales._ref, indices._ref, num_indices))
+
+    def attention_quant(self, out: CudaBuffer, q: CudaBuffer, k_pool: CudaBuffer, k_scales: CudaBuffer, v_pool: CudaBuffer,
+                        v_scales: CudaBuffer, block_table: CudaBuffer, query_starts: CudaBuffer, seq_lens: CudaBuffer,
+                        n_heads: int, n_kv_heads: int, head_dim: int, block_size: int, max_blocks_per_seq: int) -> None:
+        """`attention` over an 8-bit cache; q and out F32 or BF16, any n_heads that is a multiple of n_kv_heads."""
+        self._check(self._lib.llmrs_cuda_attention_quant(
+            self._ctx, out._ref, q._ref, k_pool._ref, k_scales._ref, v_pool._ref, v_scales._ref, block_table._ref,
+            query_starts._ref, seq_lens._ref, n_heads, n_kv_heads, head_dim, block_size, max_blocks_per_seq))
 
     def rms_norm_matmul(self, out: CudaBuffer, weight: CudaBuffer, input: CudaBuffer, norm_weight: CudaBuffer,
                         eps: float) -> None:

@@ -5,6 +5,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <cmath>
 #include <cstdarg>
 #include <cstdio>
 #include <cstdlib>
@@ -108,6 +109,7 @@ struct llmrs_ctx {
         if (code == 0) return LLMRS_OK;
         cudaMemset(dev_error, 0, 2 * sizeof code);
         if (split_ws) cudaMemset(split_ws, 0, gemm_split_counter_bytes());     // an abandoned launch may have left counters behind
+        if (code == 8) return fail(LLMRS_ERR_ARG, "%s: an index of an 8-bit cache call named a slot, page or length beyond the pool or the page table", what);
         if (code == 7) return fail(LLMRS_ERR_ARG, "%s: embed was given a token id beyond the table", what);
         return fail(LLMRS_ERR_KERNEL, "%s: a kernel gave up a bounded wait (code %u); results are incomplete", what, code);
     }
@@ -185,7 +187,7 @@ bool storage_size(uint32_t dtype, uint64_t n_elems, size_t *out) {
         *out = (size_t)(n_elems / 32) * (dtype == LLMRS_Q8_0 ? 34 : 18);
         return true;
     }
-    size_t eb = dtype == LLMRS_I32 ? 4 : dtype == LLMRS_F16 ? 2 : dense_elem_bytes(dtype);
+    size_t eb = dtype == LLMRS_I32 ? 4 : dtype == LLMRS_F16 ? 2 : dtype == LLMRS_E4M3 ? 1 : dense_elem_bytes(dtype);
     if (!eb) return false;
     *out = (size_t)n_elems * eb;
     return true;
@@ -263,6 +265,7 @@ const char *dtype_name(uint32_t dt) {
         case LLMRS_Q8_0: return "q8_0";
         case LLMRS_Q4_0: return "q4_0";
         case LLMRS_I32: return "i32";
+        case LLMRS_E4M3: return "e4m3";
         default: return "?";
     }
 }
@@ -424,8 +427,8 @@ int llmrs_cuda_alloc(llmrs_ctx *ctx, uint32_t dtype, const uint64_t *shape, int 
     if (!out) return ctx->fail(LLMRS_ERR_ARG, "alloc: out is null");
     uint32_t d0, d1;
     if (!shape_dims(shape, ndims, &d0, &d1)) return ctx->fail(LLMRS_ERR_SHAPE, "alloc: bad shape");
-    size_t eb = dtype == LLMRS_I32 ? 4 : dense_elem_bytes(dtype);
-    if (!eb) return ctx->fail(LLMRS_ERR_DTYPE, "alloc: dtype %u is not F32/BF16/I32", dtype);
+    size_t eb = dtype == LLMRS_I32 ? 4 : dtype == LLMRS_E4M3 ? 1 : dense_elem_bytes(dtype);
+    if (!eb) return ctx->fail(LLMRS_ERR_DTYPE, "alloc: dtype %u is not F32/BF16/I32/E4M3", dtype);
     size_t nbytes = (size_t)d0 * (d1 ? d1 : 1) * eb;
     DeviceGuard guard(ctx->device);
     void *p = nullptr;
@@ -440,8 +443,8 @@ int llmrs_cuda_wrap(llmrs_ctx *ctx, void *dptr, uint32_t dtype, const uint64_t *
     if (!out || !dptr) return ctx->fail(LLMRS_ERR_ARG, "wrap: null pointer");
     uint32_t d0, d1;
     if (!shape_dims(shape, ndims, &d0, &d1)) return ctx->fail(LLMRS_ERR_SHAPE, "wrap: bad shape");
-    size_t eb = dtype == LLMRS_I32 ? 4 : dense_elem_bytes(dtype);
-    if (!eb) return ctx->fail(LLMRS_ERR_DTYPE, "wrap: dtype %u is not F32/BF16/I32", dtype);
+    size_t eb = dtype == LLMRS_I32 ? 4 : dtype == LLMRS_E4M3 ? 1 : dense_elem_bytes(dtype);
+    if (!eb) return ctx->fail(LLMRS_ERR_DTYPE, "wrap: dtype %u is not F32/BF16/I32/E4M3", dtype);
     if ((uintptr_t)dptr % 16) return ctx->fail(LLMRS_ERR_ARG, "wrap: pointer must be 16-byte aligned");
     *out = llmrs_buf{dptr, (size_t)d0 * (d1 ? d1 : 1) * eb, dtype, d0, d1, LLMRS_LAYOUT_RAW, 0u,
                      (uint32_t)ctx->device};
@@ -1069,6 +1072,263 @@ int llmrs_cuda_attention(llmrs_ctx *ctx, llmrs_buf *out, const llmrs_buf *q, con
                              (int)head_dim, (int)block_size, (int)max_blocks_per_seq, ctx->stream, ctx->pdl);
     if (e != cudaSuccess) return ctx->cuda_fail(e, "attention");
     ctx->launches++;
+    return LLMRS_OK;
+}
+
+// ---- scaled rotary positions and the 8-bit KV cache ------------------------------------------------
+
+static uint32_t buf_cols(const llmrs_buf *b) { return b->dim1 ? b->dim1 : 1; }
+static bool bufs_overlap(const llmrs_buf *a, const llmrs_buf *b) {
+    const uintptr_t pa = (uintptr_t)a->dptr, pb = (uintptr_t)b->dptr;
+    return pa < pb + b->nbytes && pb < pa + a->nbytes;
+}
+// What every buffer of these calls has to be: there, on this device, 16-byte aligned.
+static int quant_bufs_ok(llmrs_ctx *ctx, const char *name, const llmrs_buf *const *bufs, int n) {
+    for (int i = 0; i < n; i++) {
+        if (!bufs[i] || !bufs[i]->dptr) return ctx->fail(LLMRS_ERR_ARG, "%s: null buffer", name);
+        if (bufs[i]->device != (uint32_t)ctx->device) return ctx->fail(LLMRS_ERR_ARG, "%s: buffers belong to another device", name);
+        if ((uintptr_t)bufs[i]->dptr & 15) return ctx->fail(LLMRS_ERR_ARG, "%s: buffers must be 16-byte aligned", name);
+    }
+    return LLMRS_OK;
+}
+// bufs[out] is an output: it may overlap none of the others, but be one of them, bufs[same] (-1: none).
+static int quant_overlap_ok(llmrs_ctx *ctx, const char *name, const llmrs_buf *const *bufs, int n, int out, int same = -1) {
+    for (int i = 0; i < n; i++)
+        if (i != out && bufs_overlap(bufs[out], bufs[i]) && !(i == same && bufs[i]->dptr == bufs[out]->dptr))
+            return ctx->fail(LLMRS_ERR_ARG, "%s: an output overlaps another buffer", name);
+    return LLMRS_OK;
+}
+// A pool and its scales: E4M3 [kv_dim, slots] and F32 [slots, n_kv_heads].
+static int quant_pool_ok(llmrs_ctx *ctx, const char *name, const llmrs_buf *pool, const llmrs_buf *scales) {
+    if (pool->dtype != LLMRS_E4M3 || scales->dtype != LLMRS_F32)
+        return ctx->fail(LLMRS_ERR_DTYPE, "%s: pools are E4M3 and their scales F32", name);
+    const uint32_t heads = buf_cols(scales);
+    if (scales->dim0 != buf_cols(pool) || pool->dim0 % heads || (pool->dim0 / heads) % 2 || pool->dim0 / heads > 256)
+        return ctx->fail(LLMRS_ERR_SHAPE, "%s: pool [%u, %u], scales [%u, %u]: scales are [slots, heads], head_dim even and at most 256",
+                         name, pool->dim0, pool->dim1, scales->dim0, scales->dim1);
+    return LLMRS_OK;
+}
+
+int llmrs_cuda_rope_frequencies(uint32_t rotary_dim, float rope_theta, const llmrs_rope_scaling *scaling,
+                                const float *factors, float *inv_freq, float *magnitude) {
+    auto bad = [](int code, const char *what) { g_create_error = what; return code; };
+    if (!inv_freq || !magnitude) return bad(LLMRS_ERR_ARG, "rope_frequencies: null pointer");
+    if (rotary_dim < 2 || rotary_dim % 2 || rotary_dim > 256)
+        return bad(LLMRS_ERR_SHAPE, "rope_frequencies: rotary_dim must be even, 2 .. 256");
+    if (!(rope_theta > 1.0f) || std::isinf(rope_theta)) return bad(LLMRS_ERR_ARG, "rope_frequencies: rope_theta must be above 1 and finite");
+    const llmrs_rope_scaling none = {LLMRS_ROPE_NONE, 0, 1.0f, 0.0f, 0.0f};
+    const llmrs_rope_scaling sc = scaling ? *scaling : none;
+    if (sc.kind > LLMRS_ROPE_YARN) return bad(LLMRS_ERR_ARG, "rope_frequencies: unknown kind of scaling");
+    if (sc.kind != LLMRS_ROPE_NONE && (!(sc.factor >= 1.0f) || std::isinf(sc.factor)))
+        return bad(LLMRS_ERR_ARG, "rope_frequencies: factor must be at least 1 and finite");
+    if ((sc.kind == LLMRS_ROPE_WAVELENGTH || sc.kind == LLMRS_ROPE_YARN) &&
+        (!sc.original_context || !(sc.low > 0.0f) || !(sc.high > sc.low) || std::isinf(sc.high)))
+        return bad(LLMRS_ERR_ARG, "rope_frequencies: original_context must be positive and 0 < low < high");
+    const uint32_t n = rotary_dim / 2;
+    for (uint32_t i = 0; factors && i < n; i++)
+        if (!(factors[i] > 0.0f) || std::isinf(factors[i])) return bad(LLMRS_ERR_ARG, "rope_frequencies: factors must be positive and finite");
+    const double two_pi = 6.283185307179586477, theta = rope_theta, ctx_len = sc.original_context;
+    // YARN: the index whose frequency makes `turns` turns over the original context
+    auto index_of = [&](double turns) { return rotary_dim * std::log(ctx_len / (turns * two_pi)) / (2.0 * std::log(theta)); };
+    double first = 0.0, last = 0.0;
+    if (sc.kind == LLMRS_ROPE_YARN) {
+        first = std::max(std::floor(index_of(sc.high)), 0.0);
+        last = std::min(std::ceil(index_of(sc.low)), (double)rotary_dim - 1.0);
+    }
+    for (uint32_t i = 0; i < n; i++) {
+        double f = std::pow(theta, -2.0 * i / rotary_dim);
+        double keep = 1.0;                               // share of f itself; the rest is f / factor
+        if (sc.kind == LLMRS_ROPE_LINEAR) keep = 0.0;
+        if (sc.kind == LLMRS_ROPE_WAVELENGTH)
+            keep = std::min(1.0, std::max(0.0, (f * ctx_len / two_pi - sc.low) / ((double)sc.high - sc.low)));
+        if (sc.kind == LLMRS_ROPE_YARN)
+            keep = last > first ? std::min(1.0, std::max(0.0, 1.0 - (i - first) / (last - first))) : i <= first ? 1.0 : 0.0;
+        f *= keep + (sc.kind == LLMRS_ROPE_NONE ? 0.0 : (1.0 - keep) / sc.factor);
+        inv_freq[i] = (float)(factors ? f / factors[i] : f);
+    }
+    *magnitude = sc.kind == LLMRS_ROPE_YARN ? (float)(1.0 + 0.1 * std::log((double)sc.factor)) : 1.0f;
+    return LLMRS_OK;
+}
+
+// q, k, positions and the table of a rotating call.
+static int rope_table_ok(llmrs_ctx *ctx, const char *name, const llmrs_buf *q, const llmrs_buf *k, const llmrs_buf *positions,
+                         const llmrs_buf *inv_freq, uint32_t head_dim, float magnitude) {
+    if (!dense_elem_bytes(q->dtype) || k->dtype != q->dtype || positions->dtype != LLMRS_I32 || inv_freq->dtype != LLMRS_F32)
+        return ctx->fail(LLMRS_ERR_DTYPE, "%s: activations of one type (F32 or BF16), positions I32, inv_freq F32", name);
+    if (head_dim == 0 || head_dim % 2 || head_dim > 256 || q->dim0 % head_dim || k->dim0 % head_dim || buf_cols(k) != buf_cols(q) ||
+        buf_elems(positions) < buf_cols(q) || inv_freq->dim1 > 1 || inv_freq->dim0 > head_dim / 2)
+        return ctx->fail(LLMRS_ERR_SHAPE, "%s: q [%u, %u], k [%u, %u], head_dim %u, %zu positions, inv_freq [%u]", name, q->dim0, q->dim1,
+                         k->dim0, k->dim1, head_dim, buf_elems(positions), inv_freq->dim0);
+    if (!std::isfinite(magnitude)) return ctx->fail(LLMRS_ERR_ARG, "%s: magnitude is not finite", name);
+    return LLMRS_OK;
+}
+
+int llmrs_cuda_rope_scaled(llmrs_ctx *ctx, llmrs_buf *q_out, llmrs_buf *k_out, const llmrs_buf *q, const llmrs_buf *k,
+                           const llmrs_buf *positions, const llmrs_buf *inv_freq, uint32_t head_dim, float magnitude,
+                           uint32_t split_half) {
+    if (!ctx) return LLMRS_ERR_ARG;
+    const char *name = "rope_scaled";
+    const llmrs_buf *all[6] = {q_out, k_out, q, k, positions, inv_freq};
+    if (int rc = quant_bufs_ok(ctx, name, all, 6)) return rc;
+    if (int rc = rope_table_ok(ctx, name, q, k, positions, inv_freq, head_dim, magnitude)) return rc;
+    if (q_out->dtype != q->dtype || k_out->dtype != k->dtype)
+        return ctx->fail(LLMRS_ERR_DTYPE, "%s: outputs have the type of q and k", name);
+    if (q_out->dim0 != q->dim0 || buf_cols(q_out) != buf_cols(q) || k_out->dim0 != k->dim0 || buf_cols(k_out) != buf_cols(k))
+        return ctx->fail(LLMRS_ERR_SHAPE, "%s: outputs have the shape of q and k", name);
+    if (int rc = quant_overlap_ok(ctx, name, all, 6, 0, 2)) return rc;
+    if (int rc = quant_overlap_ok(ctx, name, all, 6, 1, 3)) return rc;
+    DeviceGuard guard(ctx->device);
+    cudaError_t e = ctx->begin_work();
+    PerfScope perf(ctx, name, 2.0 * (buf_elems(q) + buf_elems(k)) * dense_elem_bytes(q->dtype), 0.0);
+    RopeWrite p = {};
+    p.q = q->dptr; p.k = k->dptr; p.q_out = q_out->dptr; p.k_out = k_out->dptr;
+    p.positions = (const uint32_t *)positions->dptr; p.inv_freq = (const float *)inv_freq->dptr; p.err = ctx->dev_error;
+    p.magnitude = magnitude; p.nq = (int)(q->dim0 / head_dim); p.nk = (int)(k->dim0 / head_dim);
+    p.head_dim = (int)head_dim; p.rotary = 2 * (int)inv_freq->dim0; p.split_half = split_half != 0;
+    if (e == cudaSuccess) e = launch_rope_write(p, (int)q->dtype, (int)buf_cols(q), ctx->sm_count, ctx->stream, ctx->pdl);
+    if (e != cudaSuccess) return ctx->cuda_fail(e, name);
+    ctx->launches++;
+    return LLMRS_OK;
+}
+
+int llmrs_cuda_scatter_kv_quant(llmrs_ctx *ctx, llmrs_buf *pool, llmrs_buf *scales, const llmrs_buf *src,
+                                const llmrs_buf *slot_mapping, uint32_t num_tokens) {
+    if (!ctx) return LLMRS_ERR_ARG;
+    const char *name = "scatter_kv_quant";
+    const llmrs_buf *all[4] = {pool, scales, src, slot_mapping};
+    if (int rc = quant_bufs_ok(ctx, name, all, 4)) return rc;
+    if (int rc = quant_pool_ok(ctx, name, pool, scales)) return rc;
+    if (!dense_elem_bytes(src->dtype) || slot_mapping->dtype != LLMRS_I32)
+        return ctx->fail(LLMRS_ERR_DTYPE, "%s: src F32 or BF16, slot_mapping I32", name);
+    if (src->dim0 != pool->dim0 || num_tokens > buf_cols(src) || num_tokens > buf_elems(slot_mapping))
+        return ctx->fail(LLMRS_ERR_SHAPE, "%s: %u tokens of src [%u, %u] into rows of %u, %zu slots", name, num_tokens, src->dim0,
+                         src->dim1, pool->dim0, buf_elems(slot_mapping));
+    if (int rc = quant_overlap_ok(ctx, name, all, 4, 0)) return rc;
+    if (int rc = quant_overlap_ok(ctx, name, all, 4, 1)) return rc;
+    if (num_tokens == 0) return LLMRS_OK;
+    DeviceGuard guard(ctx->device);
+    cudaError_t e = ctx->begin_work();
+    PerfScope perf(ctx, name, (double)num_tokens * (pool->dim0 * (1.0 + dense_elem_bytes(src->dtype)) + 4.0 * buf_cols(scales)), 0.0);
+    RopeWrite p = {};
+    p.v = src->dptr; p.v_pool = (uint8_t *)pool->dptr; p.v_scales = (float *)scales->dptr;
+    p.slots = (const uint32_t *)slot_mapping->dptr; p.err = ctx->dev_error; p.num_slots = buf_cols(pool);
+    p.nv = (int)buf_cols(scales); p.head_dim = (int)(pool->dim0 / buf_cols(scales));
+    if (e == cudaSuccess) e = launch_rope_write(p, (int)src->dtype, (int)num_tokens, ctx->sm_count, ctx->stream, ctx->pdl);
+    if (e != cudaSuccess) return ctx->cuda_fail(e, name);
+    ctx->launches++;
+    return LLMRS_OK;
+}
+
+int llmrs_cuda_rope_scatter_kv_quant(llmrs_ctx *ctx, llmrs_buf *q_out, const llmrs_buf *q, const llmrs_buf *k,
+                                     const llmrs_buf *v, const llmrs_buf *positions, const llmrs_buf *inv_freq,
+                                     uint32_t head_dim, float magnitude, uint32_t split_half, llmrs_buf *k_pool,
+                                     llmrs_buf *k_scales, llmrs_buf *v_pool, llmrs_buf *v_scales,
+                                     const llmrs_buf *slot_mapping) {
+    if (!ctx) return LLMRS_ERR_ARG;
+    const char *name = "rope_scatter_kv_quant";
+    const llmrs_buf *all[11] = {q_out, q, k, v, positions, inv_freq, k_pool, k_scales, v_pool, v_scales, slot_mapping};
+    if (int rc = quant_bufs_ok(ctx, name, all, 11)) return rc;
+    if (int rc = rope_table_ok(ctx, name, q, k, positions, inv_freq, head_dim, magnitude)) return rc;
+    if (int rc = quant_pool_ok(ctx, name, k_pool, k_scales)) return rc;
+    if (int rc = quant_pool_ok(ctx, name, v_pool, v_scales)) return rc;
+    if (q_out->dtype != q->dtype || v->dtype != q->dtype || slot_mapping->dtype != LLMRS_I32)
+        return ctx->fail(LLMRS_ERR_DTYPE, "%s: q_out, q, k and v of one type, slot_mapping I32", name);
+    if (q_out->dim0 != q->dim0 || buf_cols(q_out) != buf_cols(q) || v->dim0 != k->dim0 || buf_cols(v) != buf_cols(k) ||
+        buf_elems(slot_mapping) < buf_cols(q) || k_pool->dim0 != k->dim0 || v_pool->dim0 != k->dim0 ||
+        buf_cols(k_pool) != buf_cols(v_pool) || k->dim0 / buf_cols(k_scales) != head_dim || k->dim0 / buf_cols(v_scales) != head_dim)
+        return ctx->fail(LLMRS_ERR_SHAPE, "%s: q [%u, %u], k [%u, %u], v [%u, %u], pools [%u, %u] and [%u, %u], head_dim %u", name,
+                         q->dim0, q->dim1, k->dim0, k->dim1, v->dim0, v->dim1, k_pool->dim0, k_pool->dim1, v_pool->dim0,
+                         v_pool->dim1, head_dim);
+    if (int rc = quant_overlap_ok(ctx, name, all, 11, 0, 1)) return rc;
+    for (int i = 6; i < 10; i++)
+        if (int rc = quant_overlap_ok(ctx, name, all, 11, i)) return rc;
+    DeviceGuard guard(ctx->device);
+    cudaError_t e = ctx->begin_work();
+    PerfScope perf(ctx, name, (2.0 * buf_elems(q) + 2.0 * buf_elems(k)) * dense_elem_bytes(q->dtype) + 2.0 * buf_elems(k) +
+                   8.0 * buf_cols(k) * buf_cols(k_scales), 0.0);
+    RopeWrite p = {};
+    p.q = q->dptr; p.k = k->dptr; p.v = v->dptr; p.q_out = q_out->dptr;
+    p.k_pool = (uint8_t *)k_pool->dptr; p.v_pool = (uint8_t *)v_pool->dptr;
+    p.k_scales = (float *)k_scales->dptr; p.v_scales = (float *)v_scales->dptr;
+    p.positions = (const uint32_t *)positions->dptr; p.slots = (const uint32_t *)slot_mapping->dptr;
+    p.inv_freq = (const float *)inv_freq->dptr; p.err = ctx->dev_error; p.num_slots = buf_cols(k_pool);
+    p.magnitude = magnitude; p.nq = (int)(q->dim0 / head_dim); p.nk = p.nv = (int)(k->dim0 / head_dim);
+    p.head_dim = (int)head_dim; p.rotary = 2 * (int)inv_freq->dim0; p.split_half = split_half != 0;
+    if (e == cudaSuccess) e = launch_rope_write(p, (int)q->dtype, (int)buf_cols(q), ctx->sm_count, ctx->stream, ctx->pdl);
+    if (e != cudaSuccess) return ctx->cuda_fail(e, name);
+    ctx->launches++;
+    return LLMRS_OK;
+}
+
+int llmrs_cuda_gather_quant(llmrs_ctx *ctx, llmrs_buf *out, const llmrs_buf *pool, const llmrs_buf *scales,
+                            const llmrs_buf *indices, uint32_t num_indices) {
+    if (!ctx) return LLMRS_ERR_ARG;
+    const char *name = "gather_quant";
+    const llmrs_buf *all[4] = {out, pool, scales, indices};
+    if (int rc = quant_bufs_ok(ctx, name, all, 4)) return rc;
+    if (int rc = quant_pool_ok(ctx, name, pool, scales)) return rc;
+    if (!dense_elem_bytes(out->dtype) || indices->dtype != LLMRS_I32)
+        return ctx->fail(LLMRS_ERR_DTYPE, "%s: out F32 or BF16, indices I32", name);
+    if (out->dim0 != pool->dim0 || num_indices > buf_cols(out) || num_indices > buf_elems(indices))
+        return ctx->fail(LLMRS_ERR_SHAPE, "%s: %u columns of %u values into [%u, %u], %zu indices", name, num_indices, pool->dim0,
+                         out->dim0, out->dim1, buf_elems(indices));
+    if (int rc = quant_overlap_ok(ctx, name, all, 4, 0)) return rc;
+    if (num_indices == 0) return LLMRS_OK;
+    DeviceGuard guard(ctx->device);
+    cudaError_t e = ctx->begin_work();
+    PerfScope perf(ctx, name, (double)num_indices * (pool->dim0 * (1.0 + dense_elem_bytes(out->dtype)) + 4.0 * buf_cols(scales)), 0.0);
+    if (e == cudaSuccess)
+        e = launch_gather_quant(out->dptr, (int)out->dtype, (const uint8_t *)pool->dptr, (const float *)scales->dptr,
+                                (const uint32_t *)indices->dptr, pool->dim0, pool->dim0 / buf_cols(scales), buf_cols(pool),
+                                num_indices, ctx->dev_error, ctx->stream, ctx->pdl);
+    if (e != cudaSuccess) return ctx->cuda_fail(e, name);
+    ctx->launches++;
+    return LLMRS_OK;
+}
+
+int llmrs_cuda_attention_quant(llmrs_ctx *ctx, llmrs_buf *out, const llmrs_buf *q, const llmrs_buf *k_pool,
+                               const llmrs_buf *k_scales, const llmrs_buf *v_pool, const llmrs_buf *v_scales,
+                               const llmrs_buf *block_table, const llmrs_buf *query_starts, const llmrs_buf *seq_lens,
+                               uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim, uint32_t block_size,
+                               uint32_t max_blocks_per_seq) {
+    if (!ctx) return LLMRS_ERR_ARG;
+    const char *name = "attention_quant";
+    const llmrs_buf *all[9] = {out, q, k_pool, k_scales, v_pool, v_scales, block_table, query_starts, seq_lens};
+    if (int rc = quant_bufs_ok(ctx, name, all, 9)) return rc;
+    if (int rc = quant_pool_ok(ctx, name, k_pool, k_scales)) return rc;
+    if (int rc = quant_pool_ok(ctx, name, v_pool, v_scales)) return rc;
+    if (!dense_elem_bytes(q->dtype) || out->dtype != q->dtype)
+        return ctx->fail(LLMRS_ERR_DTYPE, "%s: q and out of one type (F32 or BF16)", name);
+    if (block_table->dtype != LLMRS_I32 || query_starts->dtype != LLMRS_I32 || seq_lens->dtype != LLMRS_I32)
+        return ctx->fail(LLMRS_ERR_DTYPE, "%s: block_table, query_starts and seq_lens are I32", name);
+    if (n_heads == 0 || n_kv_heads == 0 || n_heads % n_kv_heads || head_dim == 0 || head_dim % 32 || head_dim > 256 ||
+        block_size == 0 || block_size > 0x7FFFFFFFu || max_blocks_per_seq == 0 || max_blocks_per_seq > 0x7FFFFFFFu)
+        return ctx->fail(LLMRS_ERR_SHAPE, "%s: %u heads, %u kv heads, head_dim %u, pages of %u", name, n_heads, n_kv_heads,
+                         head_dim, block_size);
+    const uint64_t row = (uint64_t)n_heads * head_dim, kv_row = (uint64_t)n_kv_heads * head_dim;
+    if (k_pool->dim0 != kv_row || v_pool->dim0 != kv_row || buf_cols(k_scales) != n_kv_heads || buf_cols(v_scales) != n_kv_heads ||
+        buf_cols(k_pool) != buf_cols(v_pool))
+        return ctx->fail(LLMRS_ERR_SHAPE, "%s: pools [%u, %u] and [%u, %u], scales [%u, %u] and [%u, %u] for %u kv heads of %u", name,
+                         k_pool->dim0, k_pool->dim1, v_pool->dim0, v_pool->dim1, k_scales->dim0, k_scales->dim1, v_scales->dim0,
+                         v_scales->dim1, n_kv_heads, head_dim);
+    const uint64_t total_q = buf_elems(q) / row, num_req = buf_elems(seq_lens);
+    if (buf_elems(q) % row || buf_elems(out) != buf_elems(q) || buf_elems(query_starts) < num_req + 1 ||
+        buf_elems(block_table) / max_blocks_per_seq < num_req || total_q * n_heads > 0x7FFFFFFFull)
+        return ctx->fail(LLMRS_ERR_SHAPE, "%s: q of %zu values, %zu requests, %zu query_starts, %zu page entries", name, buf_elems(q),
+                         (size_t)num_req, buf_elems(query_starts), buf_elems(block_table));
+    if (int rc = quant_overlap_ok(ctx, name, all, 9, 0)) return rc;
+    DeviceGuard guard(ctx->device);
+    cudaError_t e = ctx->begin_work();
+    PerfScope perf(ctx, name, 2.0 * buf_elems(q) * dense_elem_bytes(q->dtype), 0.0);    // q and out: the lengths live on the device
+    AttnQuant p = {};
+    p.q = q->dptr; p.out = out->dptr; p.k_pool = (const uint8_t *)k_pool->dptr; p.v_pool = (const uint8_t *)v_pool->dptr;
+    p.k_scales = (const float *)k_scales->dptr; p.v_scales = (const float *)v_scales->dptr;
+    p.block_table = (const uint32_t *)block_table->dptr; p.query_starts = (const uint32_t *)query_starts->dptr;
+    p.seq_lens = (const uint32_t *)seq_lens->dptr; p.err = ctx->dev_error; p.num_slots = buf_cols(k_pool);
+    p.total_q = (int)total_q; p.num_req = (int)num_req; p.n_heads = (int)n_heads; p.n_kv = (int)n_kv_heads;
+    p.head_dim = (int)head_dim; p.block_size = (int)block_size; p.max_blocks = (int)max_blocks_per_seq;
+    if (e == cudaSuccess) e = launch_attention_quant(p, (int)q->dtype, ctx->stream, ctx->pdl, &ctx->launches);
+    if (e != cudaSuccess) return ctx->cuda_fail(e, name);
     return LLMRS_OK;
 }
 

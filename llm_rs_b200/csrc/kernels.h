@@ -108,6 +108,42 @@ cudaError_t launch_attention(const void *q, const void *k_pool, const void *v_po
                              int total_query_tokens, int num_requests, int n_heads, int n_kv_heads, int head_dim,
                              int block_size, int max_blocks_per_seq, cudaStream_t s, bool pdl);
 
+// ---- scaled rotary positions and the 8-bit KV cache (kv_quant.cu, attention_quant.cu) ----
+constexpr int DT_E4M3 = 256;         // codes of the 8-bit cache; not a GGUF type
+// One pass over the rows of `tokens` tokens: q and k rotated by the table inv_freq [rotary / 2] and scaled
+// by `magnitude`, q to q_out, k to k_out or (k_pool) quantised into its slot, v quantised into its slot.
+// nq, nk, nv: heads of each (0: not there).  slots null: no cache.  head_dim even, at most 256.
+struct RopeWrite {
+    const void *q, *k, *v;
+    void *q_out, *k_out;
+    uint8_t *k_pool, *v_pool;
+    float *k_scales, *v_scales;
+    const uint32_t *positions, *slots;
+    const float *inv_freq;
+    uint32_t *err;
+    uint32_t num_slots;
+    float magnitude;
+    int nq, nk, nv, head_dim, rotary, split_half;
+    int lanes_per_row;               // set by the launcher
+};
+cudaError_t launch_rope_write(const RopeWrite &p, int dtype, int tokens, int sm_count, cudaStream_t s, bool pdl);
+// out[c] (F32 or BF16) = codes * scales of slot indices[c], c < rows.
+cudaError_t launch_gather_quant(void *out, int dtype, const uint8_t *pool, const float *scales, const uint32_t *indices,
+                                uint32_t kv_dim, uint32_t head_dim, uint32_t num_slots, uint32_t rows, uint32_t *err,
+                                cudaStream_t s, bool pdl);
+// Paged attention over the 8-bit cache; the arguments of llmrs_cuda_attention_quant.
+struct AttnQuant {
+    const void *q;
+    void *out;
+    const uint8_t *k_pool, *v_pool;
+    const float *k_scales, *v_scales;
+    const uint32_t *block_table, *query_starts, *seq_lens;
+    uint32_t *err;
+    uint32_t num_slots;
+    int total_q, num_req, n_heads, n_kv, head_dim, block_size, max_blocks;
+};
+cudaError_t launch_attention_quant(const AttnQuant &p, int dtype, cudaStream_t s, bool pdl, uint64_t *launches);
+
 // Decode matmul: integer dot products per scale group, float32 across groups; any M (tokens are
 // processed in passes of <= 4).  x_dtype / out_dtype are DT_F32 or DT_BF16.  err_word names the device
 // word that receives a KernelError if a bounded wait inside the kernel gives up, and the poll limits.  *launches is

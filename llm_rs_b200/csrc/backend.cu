@@ -1318,8 +1318,6 @@ int llmrs_cuda_attention_quant(llmrs_ctx *ctx, llmrs_buf *out, const llmrs_buf *
                          (size_t)num_req, buf_elems(query_starts), buf_elems(block_table));
     if (int rc = quant_overlap_ok(ctx, name, all, 9, 0)) return rc;
     DeviceGuard guard(ctx->device);
-    cudaError_t e = ctx->begin_work();
-    PerfScope perf(ctx, name, 2.0 * buf_elems(q) * dense_elem_bytes(q->dtype), 0.0);    // q and out: the lengths live on the device
     AttnQuant p = {};
     p.q = q->dptr; p.out = out->dptr; p.k_pool = (const uint8_t *)k_pool->dptr; p.v_pool = (const uint8_t *)v_pool->dptr;
     p.k_scales = (const float *)k_scales->dptr; p.v_scales = (const float *)v_scales->dptr;
@@ -1327,7 +1325,15 @@ int llmrs_cuda_attention_quant(llmrs_ctx *ctx, llmrs_buf *out, const llmrs_buf *
     p.seq_lens = (const uint32_t *)seq_lens->dptr; p.err = ctx->dev_error; p.num_slots = buf_cols(k_pool);
     p.total_q = (int)total_q; p.num_req = (int)num_req; p.n_heads = (int)n_heads; p.n_kv = (int)n_kv_heads;
     p.head_dim = (int)head_dim; p.block_size = (int)block_size; p.max_blocks = (int)max_blocks_per_seq;
-    if (e == cudaSuccess) e = launch_attention_quant(p, (int)q->dtype, ctx->stream, ctx->pdl, &ctx->launches);
+    const size_t need = attention_quant_workspace(p, (int)q->dtype, ctx->sm_count);
+    cudaError_t e = ctx->grow((void **)&ctx->att_ws, &ctx->att_ws_bytes, need);
+    if (e == cudaErrorStreamCaptureUnsupported)
+        return ctx->fail(LLMRS_ERR_CUDA, "%s: workspace must grow (make one call outside graph capture)", name);
+    if (e != cudaSuccess) return ctx->cuda_fail(e, "attention_quant: workspace");
+    e = ctx->begin_work();
+    PerfScope perf(ctx, name, 2.0 * buf_elems(q) * dense_elem_bytes(q->dtype), 0.0);    // q and out: the lengths live on the device
+    if (e == cudaSuccess)
+        e = launch_attention_quant(p, (int)q->dtype, ctx->att_ws, ctx->sm_count, ctx->stream, ctx->pdl, &ctx->launches);
     if (e != cudaSuccess) return ctx->cuda_fail(e, name);
     return LLMRS_OK;
 }

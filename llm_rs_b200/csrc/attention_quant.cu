@@ -11,6 +11,7 @@
 #include "kernels.h"
 #include "llmrs_common.cuh"
 #include "pipeline.cuh"
+#include "tensor_map.h"
 
 namespace llmrs {
 
@@ -28,6 +29,10 @@ __device__ __forceinline__ float4 load4(const void *p, size_t i, int bf16) {
     const uint2 u = *reinterpret_cast<const uint2 *>((const uint16_t *)p + i);
     return make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xFFFF0000u), __uint_as_float(u.y << 16),
                        __uint_as_float(u.y & 0xFFFF0000u));
+}
+__device__ __forceinline__ void store2(void *p, size_t i, float2 v, int bf16) {
+    if (bf16) *reinterpret_cast<__nv_bfloat162 *>((__nv_bfloat16 *)p + i) = __floats2bfloat162_rn(v.x, v.y);
+    else *reinterpret_cast<float2 *>((float *)p + i) = v;
 }
 __device__ __forceinline__ void store4(void *p, size_t i, float4 v, int bf16) {
     if (bf16) {
@@ -150,22 +155,32 @@ __global__ void __launch_bounds__(AQ_TILE) attention_quant_simple_kernel(const A
 // long request spreads over the whole GPU.  The lengths are on the device, so each CTA adds them up itself.  A row
 // block that lies in several ranges leaves (accumulator, maximum, sum) in the workspace for the merge kernel.
 //
-// A CTA has 8 warps, HW heads x PW runs of 16 positions, so that neighbouring heads of a slot, neighbours in memory,
-// are read at the same time.  Each warp is on its own: it fetches its 16 positions NST units ahead into its own
-// ring by 16-byte asynchronous copies, and meets other warps only at the end of a row block.
+// A CTA has 8 consumer warps, HW heads x PW runs of 16 positions, so that neighbouring heads of a slot, neighbours
+// in memory, are read at the same time, and a producer that keeps NST units in flight, through to the end of the
+// CTA's range.  Where 16 positions never straddle a page (block_size a multiple of 16, and the scales' rows 16-byte
+// aligned) the producer is one thread that issues four tiled TMA copies per 16 positions of all the heads; otherwise
+// four warps fetch 16 bytes a lane.  (The first form had every warp fetch for itself: 692 instructions a warp per 16
+// positions, and one request of 131071 positions took 88 us, bound by issue slots at 48 % of HBM.)
 //
 // Arithmetic (mma m16n8k16, f16 operands, float32 sums): E4M3 codes are exact in f16; bf16 queries are too, once a row is
-// scaled by a power of two.  TERMS = 2 (F32) splits queries and weights into a high and a low f16.  The order in which
-// dimensions enter a dot product is free as long as both operands agree, so a lane takes 16 consecutive codes of a
-// row as its part of four products; codes of values come transposed by ldmatrix in pairs of dimensions, which one
-// byte permute turns into pairs of positions.  A weight enters as w = e^(s - m) vs / R * 2^15 with R the least power of two
-// that no vs so far exceeds: f16 keeps it to 2^-11 (bf16: 2^-8), and down to 2^-40 of the largest.
-constexpr int SH_WARPS = 8, SH_THREADS = 32 * SH_WARPS;
+// scaled by a power of two.  TERMS = 2 (F32) splits queries and weights into a high and a low f16.  Positions (for the
+// second product: dimensions) are the 16 rows of an operand and query rows the 8 columns, so 8 rows need one
+// product for what would take two the other way round; the weights change sides by movmatrix.  The order in
+// which dimensions enter a dot product is free as long as both operands agree, so a lane takes 16 consecutive codes
+// of a row as its part of four products; codes of values come transposed by ldmatrix in pairs of dimensions, which
+// one byte permute turns into pairs of positions.  A weight enters as w = e^(s - m) vs / R * 2^15 with R the least power
+// of two that no vs so far exceeds: f16 keeps it to 2^-11 (bf16: 2^-8), and down to 2^-40 of the largest.
+constexpr int SH_WARPS = 4, SH_THREADS = 32 * SH_WARPS;      // consumers
+constexpr int SH_GR = 2;             // runs of 16 positions that a warp takes at a time
+constexpr int SH_TILES = SH_WARPS * SH_GR;                   // (run, head) tiles of a unit
 constexpr int SH_MIN_UNITS = 4;      // a CTA gets at least this many units: shorter ranges cost more in merging than they save
 
-template <int HD> struct ShortStage {
-    static constexpr int K = 0, V = 16 * HD, KS = 32 * HD, VS = KS + 64, MASK = VS + 64, BYTES = MASK + 16;
+template <int HD, int HW> struct ShortStage {
+    static constexpr int RUNS = SH_TILES / HW, TILE = SH_TILES * 16 * HD, BYTES = 2 * TILE;   // codes: keys, then values
+    // scales (RUN bytes for 16 positions of HW heads; a TMA copy starts on 128 bytes) and which positions are there
+    static constexpr int RUN = HW == 1 ? 128 : 64 * HW, KS = 0, VS = RUNS * RUN, MASK = 2 * VS, AUX = MASK + 128;
 };
+struct ShortMaps { CUtensorMap k, v, ks, vs; };
 
 struct Rows {                        // what both kernels need to know about the split into rows and units
     int rb, tp, hw, only_short;      // rows per block, positions per unit, KV heads per CTA, leave requests of more than SHORT_ROWS rows out
@@ -230,10 +245,10 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], u
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// Two E4M3 codes (low, high byte) -> f16x2, exact.
-__device__ __forceinline__ uint32_t codes_to_f16(uint32_t two) {
-    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)two, __NV_E4M3);
-    return (uint32_t)h.x | (uint32_t)h.y << 16;
+// Four E4M3 codes -> two f16x2 (low bytes first), exact.
+__device__ __forceinline__ void codes_to_f16(uint32_t codes, uint32_t &lo, uint32_t &hi) {
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+        : "=r"(lo), "=r"(hi) : "r"(codes));
 }
 __device__ __forceinline__ float ex2(float x) {
     float r;
@@ -256,9 +271,24 @@ __device__ __forceinline__ void copy16_or_zero(void *dst, const void *src, bool 
 __device__ __forceinline__ void copy4_or_zero(void *dst, const void *src, bool on) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(on ? 4 : 0) : "memory");
 }
+// Arrives on `bar` (one of its expected arrivals) once this thread's copies so far have landed.
+__device__ __forceinline__ void copies_arrive(uint64_t *bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void tma_load_3d(void *dst, const void *tmap, int c0, int c1, int c2, uint64_t *bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+        ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(tmap)), "r"(c0), "r"(c1), "r"(c2), "r"(smem_u32(bar))
+        : "memory");
+}
 __device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&r)[4], const void *row) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(smem_u32(row)));
+}
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {             // of an 8x8 matrix of 16-bit values
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+    return r;
 }
 // The power of two by which a row of queries with largest magnitude `amax` enters as f16 (its largest then in
 // [2^13, 2^14)): 2^e, |e| <= 126.  Rows of zeros and rows that are not finite stay as they are.
@@ -266,316 +296,449 @@ __device__ __forceinline__ int row_exponent(float amax) {
     const int e = (int)(__float_as_uint(amax) >> 23);    // biased; amax >= 0
     return amax == 0.0f || e == 255 ? 0 : max(-126, min(126, 13 - (e - 127)));
 }
+// 16-byte chunk c of row `row` of a tile of HD-byte rows, as the 128- and 64-byte swizzles of TMA place it.
+template <int HD> __device__ __forceinline__ int chunk_at(int row, int c) {
+    return row * HD + 16 * (c ^ (HD == 128 ? row & 7 : (row >> 1) & 3));
+}
 
-template <int HD, int RB, int TERMS, int HW, int NST>
-__global__ void __launch_bounds__(SH_THREADS, RB == 8 && TERMS == 1 ? 2 : 1)
-attention_quant_short_kernel(const AttnQuant p, int bf16, int only_short, float *__restrict__ ws) {
-    pdl_prologue();
-    using St = ShortStage<HD>;
-    constexpr int PW = SH_WARPS / HW, TP = 16 * PW, KS = HD / 16, CH = HD / 16;
-    constexpr int HALVES = RB / 8;                       // 8 rows: the lower half of the 16-row operand stays zero
-    extern __shared__ __align__(128) uint8_t sh_smem[];
-    __shared__ long long sums[SH_WARPS], found[2];
+// A CTA's way through its range of units: one row block (or the part of it in the range) after the other.
+struct Segment {
+    Request r;
+    int req, rb, t0, t1, tiles, n_rows, kv_end, n_steps;
+    bool first;                      // starts where the range starts
+};
+template <int RB, int TP> struct Walk {
+    long long u, u_begin, u_end, req_base;
+    int req;
+    __device__ __forceinline__ bool next(const AttnQuant &p, const Rows &w, Segment &s) {
+        while (u < u_end) {
+            int blocks;
+            s.r = request_of(p, req);
+            shape_of(p, w, s.r, blocks, s.tiles);
+            if (u >= req_base + (long long)blocks * s.tiles) { req_base += (long long)blocks * s.tiles; req++; continue; }
+            const int group = p.n_heads / p.n_kv;
+            s.req = req;
+            s.rb = (int)((u - req_base) / s.tiles);
+            s.t0 = (int)((u - req_base) % s.tiles);
+            s.t1 = (int)min((long long)s.tiles, s.t0 + (u_end - u));
+            s.n_rows = min(RB, s.r.count * group - s.rb * RB);
+            s.kv_end = s.r.before + (s.rb * RB + s.n_rows - 1) / group + 1;
+            s.n_steps = max(0, min(s.t1, (max(s.kv_end, 0) + TP - 1) / TP) - s.t0);   // 0: nothing to see in this range
+            s.first = u == u_begin;
+            u += s.t1 - s.t0;
+            return true;
+        }
+        return false;
+    }
+};
+
+template <int HD, int RB, int TERMS, int HW, int NST, bool TMA>
+__global__ void __launch_bounds__(SH_THREADS + (TMA ? 32 : 128), 2)
+attention_quant_short_kernel(const __grid_constant__ ShortMaps maps, const AttnQuant p, int bf16, int only_short, uint32_t polls,
+                             float *__restrict__ ws) {
+    using St = ShortStage<HD, HW>;
+    constexpr int PW = SH_WARPS / HW, RUNS = St::RUNS, TP = 16 * RUNS, KS = HD / 16, CH = HD / 16, NT = RB / 8;
+    constexpr int PASS = 1;                              // chunks of 16 dimensions the warps of a head exchange at a time
+    extern __shared__ __align__(1024) uint8_t sh_smem[];
+    uint8_t *codes = sh_smem, *aux = codes + NST * St::BYTES;
+    float *meet = reinterpret_cast<float *>(aux + NST * St::AUX);            // PW > 1: [warp][row][16 PASS] and [warp][row] {max, sum}
+    __shared__ __align__(8) uint64_t full[NST], empty[NST];
+    __shared__ long long sums[(SH_THREADS + (TMA ? 32 : 128)) / 32], found[2];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+    if (tid == 0) {
+        for (int i = 0; i < NST; i++) {
+            mbar_init(&full[i], TMA ? 1 : 128 + 4);
+            mbar_init(&empty[i], SH_WARPS);
+        }
+        mbar_init_fence();
+    }
+    pdl_prologue();
     const int groups = p.n_kv / HW, hg = blockIdx.x % groups, cta = blockIdx.x / groups, ctas = gridDim.x / groups;
-    const int kvh = hg * HW + warp / PW, wp = warp % PW;
     const int group = p.n_heads / p.n_kv;
     const Rows rows{RB, TP, HW, only_short};
-    found[0] = -1;
     int n_cta = 1;
     const long long total = scan_units(p, rows, sums, found, [&](long long all) {
         n_cta = sharers(all, ctas);
         return cta < n_cta ? first_unit(all, n_cta, cta) : -1ll;
-    }, -1);
+    }, -1);                                              // its barriers also publish the mbarriers
     if (cta >= n_cta || total == 0) return;
-    const long long u_begin = first_unit(total, n_cta, cta), u_end = first_unit(total, n_cta, cta + 1);
-    int req = (int)found[0];
-    long long req_base = found[1];                       // units before request `req`
+    Walk<RB, TP> walk;
+    walk.u = walk.u_begin = first_unit(total, n_cta, cta);
+    walk.u_end = first_unit(total, n_cta, cta + 1);
+    walk.req = (int)found[0];
+    walk.req_base = found[1];
+    Segment s;
+    int stage = 0;
+    uint32_t phase = 0;
+    bool dead = false;                                   // a wait was given up: go on without waiting, so that no barrier is missed
 
-    uint8_t *ring = sh_smem + (size_t)warp * NST * St::BYTES;
-    const size_t kv_dim = (size_t)p.n_kv * HD;
-    const uint8_t *kp = p.k_pool + (size_t)kvh * HD, *vp = p.v_pool + (size_t)kvh * HD;
-    const float *ksp = p.k_scales + (size_t)kvh * p.num_slots, *vsp = p.v_scales + (size_t)kvh * p.num_slots;
+    if (warp >= SH_WARPS) {
+        // ---- producer ----
+        int issued = 0;
+        while (!dead && walk.next(p, rows, s)) {
+            const uint32_t *table = p.block_table + (size_t)s.req * p.max_blocks;
+            if constexpr (TMA) {
+                // lane x looks up run `r0 + x` of the segment (16 positions each, RUNS to a step); the copies then go out in order
+                for (int r0 = 0; r0 < s.n_steps * RUNS && !dead; r0 += 32) {
+                    const int pos = s.t0 * TP + 16 * (r0 + lane);
+                    int slot = (int)p.num_slots, n_ok = 0;               // out of range: zeros, nothing read
+                    if (r0 + lane < s.n_steps * RUNS && pos < s.kv_end) {
+                        const unsigned long long s64 = (unsigned long long)table[pos / p.block_size] * p.block_size + (unsigned)(pos % p.block_size);
+                        const int want = min(16, s.kv_end - pos);
+                        if (s64 < p.num_slots) { slot = (int)s64; n_ok = (int)min((unsigned long long)want, p.num_slots - s64); }
+                        if (n_ok < want) report_error(p.err, KERR_SLOT_RANGE);
+                    }
+                    const int steps = min(32 / RUNS, s.n_steps - r0 / RUNS);
+                    for (int i = 0; i < steps && !dead; i++) {
+                        if (issued >= NST && !mbar_wait(&empty[stage], phase ^ 1, polls)) { dead = true; report_error(p.err, KERR_EMPTY_WAIT); break; }
+                        uint8_t *cd = codes + stage * St::BYTES, *ax = aux + stage * St::AUX;
+                        if (lane / RUNS == i) reinterpret_cast<uint32_t *>(ax + St::MASK)[lane % RUNS] = (1u << n_ok) - 1;
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive_expect_tx(&full[stage], St::BYTES + 2 * SH_TILES * 64);
+                        __syncwarp();
+#pragma unroll
+                        for (int x = 0; x < RUNS; x++) {
+                            const int at = __shfl_sync(0xffffffffu, slot, i * RUNS + x);
+                            if (lane == 0) {
+                                tma_load_3d(cd + x * HW * 16 * HD, &maps.k, 0, at, hg * HW, &full[stage]);
+                                tma_load_3d(cd + St::TILE + x * HW * 16 * HD, &maps.v, 0, at, hg * HW, &full[stage]);
+                                tma_load_2d(ax + St::KS + x * St::RUN, &maps.ks, at, hg * HW, &full[stage]);
+                                tma_load_2d(ax + St::VS + x * St::RUN, &maps.vs, at, hg * HW, &full[stage]);
+                            }
+                        }
+                        issued++;
+                        if (++stage == NST) { stage = 0; phase ^= 1; }
+                    }
+                }
+            } else {
+                // four warps, two of the eight tiles of 16 positions each
+                const size_t kv_dim = (size_t)p.n_kv * HD;
+                const int pw = warp - SH_WARPS, j = lane & 15;
+                auto page_of = [&](int i, int run) -> uint32_t {
+                    const int pos = (s.t0 + i) * TP + run * 16 + j;
+                    return i < s.n_steps && pos < s.kv_end ? table[pos / p.block_size] : 0u;
+                };
+                uint32_t page[2] = {page_of(0, 2 * pw / HW), page_of(0, (2 * pw + 1) / HW)};
+                for (int i = 0; i < s.n_steps; i++) {
+                    if (issued >= NST && !mbar_wait(&empty[stage], phase ^ 1, polls)) { dead = true; report_error(p.err, KERR_EMPTY_WAIT); break; }
+                    uint8_t *cd = codes + stage * St::BYTES, *ax = aux + stage * St::AUX;
+#pragma unroll
+                    for (int y = 0; y < 2; y++) {
+                        const int sub = 2 * pw + y, run = sub / HW, head = hg * HW + sub % HW;
+                        const int pos = (s.t0 + i) * TP + run * 16 + j;
+                        const unsigned long long s64 = (unsigned long long)page[y] * p.block_size + (unsigned)(pos % p.block_size);
+                        const bool ok = pos < s.kv_end && s64 < p.num_slots;
+                        if (pos < s.kv_end && !ok) report_error(p.err, KERR_SLOT_RANGE);
+                        const uint32_t slot = ok ? (uint32_t)s64 : 0u;
+                        const uint32_t mask = __ballot_sync(0xffffffffu, ok) & 0xFFFFu;
+                        if (lane == 0) reinterpret_cast<uint32_t *>(ax + St::MASK)[sub] = mask;
+                        copy4_or_zero(ax + (lane < 16 ? St::KS : St::VS) + run * St::RUN + sub % HW * 64 + 4 * j,
+                                      (lane < 16 ? p.k_scales : p.v_scales) + (size_t)head * p.num_slots + slot, ok);
+                        constexpr int RPI = 32 / CH;     // rows per pass of the warp
+                        const int c = lane % CH;
+#pragma unroll
+                        for (int k = 0; k < 16 / RPI; k++) {
+                            const int row = lane / CH + RPI * k;
+                            const size_t off = (size_t)__shfl_sync(0xffffffffu, slot, row) * kv_dim + (size_t)head * HD + 16 * c;
+                            const bool on = mask >> row & 1;
+                            copy16_or_zero(cd + sub * 16 * HD + chunk_at<HD>(row, c), p.k_pool + off, on);
+                            copy16_or_zero(cd + St::TILE + sub * 16 * HD + chunk_at<HD>(row, c), p.v_pool + off, on);
+                        }
+                        page[y] = page_of(i + 1, run);
+                    }
+                    copies_arrive(&full[stage]);
+                    if (lane == 0) mbar_arrive(&full[stage]);            // the masks
+                    issued++;
+                    if (++stage == NST) { stage = 0; phase ^= 1; }
+                }
+            }
+        }
+        // no copy may be in flight when the CTA ends: the last ones issued have landed once their barriers have turned
+        for (int i = 0; i < min(issued, NST); i++) {
+            if (stage-- == 0) { stage = NST - 1; phase ^= 1; }
+            mbar_wait(&full[stage], phase, polls);
+        }
+        return;
+    }
 
-    for (long long u = u_begin; u < u_end;) {
-        int blocks, tiles;
-        const Request r = request_of(p, req);
-        shape_of(p, rows, r, blocks, tiles);
-        if (u >= req_base + (long long)blocks * tiles) { req_base += (long long)blocks * tiles; req++; continue; }
-        const int rb = (int)((u - req_base) / tiles), t0 = (int)((u - req_base) % tiles);
-        const int t1 = (int)min((long long)tiles, t0 + (u_end - u));
-        // ---- the rows of this block: rows g and g + 8 are this lane's ----
-        const int n_rows = min(RB, r.count * group - rb * RB);
-        const int kv_end = r.before + (rb * RB + n_rows - 1) / group + 1;
-        int len[2];
-        size_t q_off[2];
-        uint32_t qa[TERMS][KS][4];
-        float c_row[2];                                  // what turns a product of codes into a score in units of log2
+    // ---- consumers ----
+    constexpr int GR = SH_GR;
+    const int hw = warp % HW, wp = warp / HW, kvh = hg * HW + hw, first_tile = wp * GR * HW + hw;
+    while (walk.next(p, rows, s)) {
+        // rows: this lane loads the queries of row g (and g + 8) as operand columns; scores and sums come out for rows 2t, 2t + 1 (+ 8)
+        uint32_t qb[TERMS][NT][KS][2];
+        float c_row[NT][2];                              // what turns a product of codes into a score in units of log2
+        int len[NT][2];
+        const int min_len = s.r.before + s.rb * RB / group + 1;          // what the first row sees
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-            const int i = g + 8 * h, rr = rb * RB + i;
-            const bool on = h < HALVES && i < n_rows;
-            len[h] = on ? r.before + rr / group + 1 : 0;
-            q_off[h] = on ? ((size_t)(r.first + rr / group) * p.n_heads + (size_t)kvh * group + rr % group) * HD : 0;
-            c_row[h] = 0.0f;
-#pragma unroll
-            for (int x = 0; x < TERMS; x++)
-#pragma unroll
-                for (int ks = 0; ks < KS; ks++) qa[x][ks][h] = qa[x][ks][2 + h] = 0u;
-            if (h >= HALVES) continue;
+        for (int n = 0; n < NT; n++) {
+            const int i = g + 8 * n, rr = s.rb * RB + i;
+            const bool on = i < s.n_rows;
+            const size_t off = on ? ((size_t)(s.r.first + rr / group) * p.n_heads + (size_t)kvh * group + rr % group) * HD : 0;
+            float q[KS][4], amax = 0.0f;
             // the lane's dimensions: 16 (t + 4 hf) + 4 w + (0 .. 3) of step 4 hf + w
-            float amax = 0.0f;
-            float q[KS][4];
 #pragma unroll
             for (int ks = 0; ks < KS; ks++) {
-                const float4 v = on ? load4(p.q, q_off[h] + 16 * (t + 4 * (ks / 4)) + 4 * (ks % 4), bf16) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                const float4 v = on ? load4(p.q, off + 16 * (t + 4 * (ks / 4)) + 4 * (ks % 4), bf16) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                 q[ks][0] = v.x; q[ks][1] = v.y; q[ks][2] = v.z; q[ks][3] = v.w;
                 amax = fmaxf(amax, fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
             }
             amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
             amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
             const int ex = row_exponent(amax);
-            const float up = exp2i(ex);
-            c_row[h] = exp2i(-ex) * (1.4426950408889634f / sqrtf((float)HD));
+            const float up = exp2i(ex), c = exp2i(-ex) * (1.4426950408889634f / sqrtf((float)HD));
+            const int visible = on ? s.r.before + rr / group + 1 : 0;
+#pragma unroll
+            for (int e = 0; e < 2; e++) {                // row 2t + e is lane 4 (2t + e)'s
+                c_row[n][e] = __shfl_sync(0xffffffffu, c, 4 * (2 * t + e));
+                len[n][e] = __shfl_sync(0xffffffffu, visible, 4 * (2 * t + e));
+            }
 #pragma unroll
             for (int ks = 0; ks < KS; ks++)
 #pragma unroll
                 for (int e = 0; e < 2; e++) {
                     const float a = q[ks][2 * e] * up, b = q[ks][2 * e + 1] * up;
-                    qa[0][ks][h + 2 * e] = pack_f16(a, b);
-                    if (TERMS == 2) qa[TERMS - 1][ks][h + 2 * e] = pack_f16_rest(a, b, qa[0][ks][h + 2 * e]);
+                    qb[0][n][ks][e] = pack_f16(a, b);
+                    if (TERMS == 2) qb[TERMS - 1][n][ks][e] = pack_f16_rest(a, b, qb[0][n][ks][e]);
                 }
         }
-        float o[CH][2][4];                               // [chunk of 16 dims][even, odd dims][row g: 4t + par, 4t + 2 + par; row g + 8]
+        // [rows 8n ..][chunk of 16 dims]: dims 16c + 2g (0, 1) and 16c + 2g + 1 (2, 3) of rows 2t (0, 2) and 2t + 1 (1, 3)
+        float o[NT][CH][4];
+        float m[NT][2], l[NT][2];
 #pragma unroll
-        for (int c = 0; c < CH; c++)
+        for (int n = 0; n < NT; n++) {
+            m[n][0] = m[n][1] = -INFINITY;
+            l[n][0] = l[n][1] = 0.0f;
 #pragma unroll
-            for (int x = 0; x < 2; x++) o[c][x][0] = o[c][x][1] = o[c][x][2] = o[c][x][3] = 0.0f;
-        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+            for (int c = 0; c < CH; c++) o[n][c][0] = o[n][c][1] = o[n][c][2] = o[n][c][3] = 0.0f;
+        }
         uint32_t r_bits = 17u << 23;                     // R: a power of two, at least 2^-110
 
-        const int n_steps = min(t1, (max(kv_end, 0) + TP - 1) / TP) - t0;        // at most 0: nothing to see in this range
-        const int j = lane & 15;
-        auto page_of = [&](int i) -> uint32_t {          // page table entry of this lane's position of step i
-            const int pos = (t0 + i) * TP + wp * 16 + j;
-            return i < n_steps && pos < kv_end ? p.block_table[(size_t)req * p.max_blocks + pos / p.block_size] : 0u;
-        };
-        uint32_t page = page_of(0);
-        auto fetch = [&](int i) {
-            if (i < n_steps) {
-                uint8_t *st = ring + (i % NST) * St::BYTES;
-                const int pos = (t0 + i) * TP + wp * 16 + j;
-                const unsigned long long s64 = (unsigned long long)page * p.block_size + (unsigned)(pos % p.block_size);
-                const bool ok = pos < kv_end && s64 < p.num_slots;
-                if (pos < kv_end && !ok) report_error(p.err, KERR_SLOT_RANGE);
-                const uint32_t slot = ok ? (uint32_t)s64 : 0u;
-                const uint32_t mask = __ballot_sync(0xffffffffu, ok) & 0xFFFFu;
-                if (lane == 0) *reinterpret_cast<uint32_t *>(st + St::MASK) = mask;
-                copy4_or_zero(st + (lane < 16 ? St::KS : St::VS) + 4 * j, (lane < 16 ? ksp : vsp) + slot, ok);
-                constexpr int RPI = 32 / CH;             // rows per pass of the warp
-                const int c = lane % CH;
+        for (int i = 0; i < s.n_steps; i++) {
+            if (!dead && !mbar_wait(&full[stage], phase, polls)) { dead = true; report_error(p.err, KERR_FULL_WAIT); }
+            uint8_t *kt = codes + stage * St::BYTES + first_tile * 16 * HD, *vt = kt + St::TILE;
+            const uint8_t *ax = aux + stage * St::AUX;
+            const int p0 = (s.t0 + i) * TP + wp * 16 * GR;
+            uint32_t mask[GR];
+            float kw[GR][2], vw[GR][2];                  // scales of positions g and g + 8 of each run
+            bool all = p0 + 16 * GR <= min_len;          // every row sees every position
 #pragma unroll
-                for (int k = 0; k < 16 / RPI; k++) {
-                    const int row = lane / CH + RPI * k;
-                    const size_t off = (size_t)__shfl_sync(0xffffffffu, slot, row) * kv_dim + 16 * c;
-                    const bool on = mask >> row & 1;
-                    // chunks of a row are permuted so that fragment reads fall on distinct banks
-                    copy16_or_zero(st + St::K + row * HD + 16 * (c ^ (HD == 128 ? (row & 1) << 2 : 0)), kp + off, on);
-                    copy16_or_zero(st + St::V + row * HD + 16 * (c ^ (HD == 128 ? row & 7 : (row >> 1) & 3)), vp + off, on);
-                }
-                page = page_of(i + 1);
+            for (int r = 0; r < GR; r++) {
+                mask[r] = reinterpret_cast<const uint32_t *>(ax + St::MASK)[TMA ? wp * GR + r : first_tile + r * HW];
+                all = all && mask[r] == 0xFFFFu;
+                const float *ks = reinterpret_cast<const float *>(ax + (wp * GR + r) * St::RUN) + 16 * hw, *vs = ks + St::VS / 4;
+                kw[r][0] = ks[g]; kw[r][1] = ks[g + 8];
+                vw[r][0] = vs[g]; vw[r][1] = vs[g + 8];
             }
-            asm volatile("cp.async.commit_group;" ::: "memory");
-        };
+            // ---- scores: positions g and g + 8 of each run against rows 2t, 2t + 1 ----
+            float sc[GR][NT][4];
 #pragma unroll
-        for (int i = 0; i < NST - 1; i++) fetch(i);
-        for (int i = 0; i < n_steps; i++) {
-            asm volatile("cp.async.wait_group %0;" ::"n"(NST - 2) : "memory");
-            __syncwarp();                                // this step's bytes are there for all lanes, the last step's are no longer read
-            fetch(i + NST - 1);
-            const uint8_t *st = ring + (i % NST) * St::BYTES;
-            // ---- scores of the warp's 16 positions: two groups of eight ----
-            float s[2][4];
+            for (int r = 0; r < GR; r++) {
 #pragma unroll
-            for (int nt = 0; nt < 2; nt++) {
-                s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.0f;
-                const int row = 8 * nt + g;
+                for (int n = 0; n < NT; n++) sc[r][n][0] = sc[r][n][1] = sc[r][n][2] = sc[r][n][3] = 0.0f;
 #pragma unroll
                 for (int hf = 0; hf < KS / 4; hf++) {
-                    const int c = HD == 128 ? (t + 4 * hf) ^ ((row & 1) << 2) : t;
-                    const uint4 w4 = *reinterpret_cast<const uint4 *>(st + St::K + row * HD + 16 * c);
-                    const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+                    const uint4 wa = *reinterpret_cast<const uint4 *>(kt + r * HW * 16 * HD + chunk_at<HD>(g, t + 4 * hf));
+                    const uint4 wb = *reinterpret_cast<const uint4 *>(kt + r * HW * 16 * HD + chunk_at<HD>(g + 8, t + 4 * hf));
+                    const uint32_t w0[4] = {wa.x, wa.y, wa.z, wa.w}, w1[4] = {wb.x, wb.y, wb.z, wb.w};
 #pragma unroll
                     for (int x = 0; x < 4; x++) {
-                        const uint32_t b0 = codes_to_f16(w[x] & 0xFFFFu), b1 = codes_to_f16(w[x] >> 16);
+                        uint32_t a[4];
+                        codes_to_f16(w0[x], a[0], a[2]);
+                        codes_to_f16(w1[x], a[1], a[3]);
 #pragma unroll
-                        for (int y = 0; y < TERMS; y++) mma_f16(s[nt], qa[y][4 * hf + x], b0, b1);
+                        for (int n = 0; n < NT; n++)
+#pragma unroll
+                            for (int y = 0; y < TERMS; y++) mma_f16(sc[r][n], a, qb[y][n][4 * hf + x][0], qb[y][n][4 * hf + x][1]);
                     }
                 }
             }
-            const uint32_t mask = *reinterpret_cast<const uint32_t *>(st + St::MASK);
-            const float *ks = reinterpret_cast<const float *>(st + St::KS), *vs = reinterpret_cast<const float *>(st + St::VS);
-            float vw[2][2], vmax = 0.0f;
-            const int p0 = (t0 + i) * TP + wp * 16;
-            float mx[2] = {-INFINITY, -INFINITY};
-            bool seen[2][2][2];                          // [half][group][element]
+            // ---- what a row does not see, the running maxima, the size of the values, the weights ----
 #pragma unroll
-            for (int nt = 0; nt < 2; nt++) {
-                const float2 k2 = *reinterpret_cast<const float2 *>(ks + 8 * nt + 2 * t), v2 = *reinterpret_cast<const float2 *>(vs + 8 * nt + 2 * t);
+            for (int r = 0; r < GR; r++)
+#pragma unroll
+                for (int n = 0; n < NT; n++)
+#pragma unroll
+                    for (int x = 0; x < 4; x++) sc[r][n][x] *= kw[r][x >> 1] * c_row[n][x & 1];
+            if (!all) {
+#pragma unroll
+                for (int r = 0; r < GR; r++) {
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        const bool ok = mask[r] >> (g + 8 * h) & 1;
+                        if (!ok) vw[r][h] = 0.0f;
+#pragma unroll
+                        for (int n = 0; n < NT; n++)
+#pragma unroll
+                            for (int e = 0; e < 2; e++)
+                                if (!ok || p0 + 16 * r + g + 8 * h >= len[n][e]) sc[r][n][2 * h + e] = -INFINITY;
+                    }
+                    if (TMA && mask[r] != 0xFFFFu) {     // rows of no position: their weight is zero, but their bytes may be NaN codes
+                        uint8_t *v = vt + r * HW * 16 * HD;
+                        for (int row = __popc(mask[r]) + lane / CH; row < 16; row += 32 / CH)
+                            *reinterpret_cast<uint4 *>(v + row * HD + 16 * (lane % CH)) = make_uint4(0, 0, 0, 0);
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // before a copy writes there again
+                    }
+                }
+                __syncwarp();
+            }
+            float vmax = 0.0f;
+#pragma unroll
+            for (int r = 0; r < GR; r++) vmax = fmaxf(vmax, fmaxf(vw[r][0], vw[r][1]));
+#pragma unroll
+            for (int x = 4; x <= 16; x <<= 1) vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, x));
+            const uint32_t r_new = max(r_bits, min((__float_as_uint(vmax) + 0x7FFFFFu) & 0x7F800000u, 253u << 23));
+            bool moved = r_new != r_bits;
+            float f[NT][2], top[NT][2];
+#pragma unroll
+            for (int n = 0; n < NT; n++)
 #pragma unroll
                 for (int e = 0; e < 2; e++) {
-                    const int at = 8 * nt + 2 * t + e;
-                    const bool ok = mask >> at & 1;
-                    vw[nt][e] = e ? v2.y : v2.x;
-                    vmax = fmaxf(vmax, vw[nt][e]);
+                    float mx = fmaxf(sc[0][n][e], sc[0][n][2 + e]);
 #pragma unroll
-                    for (int h = 0; h < HALVES; h++) {
-                        seen[h][nt][e] = ok && p0 + at < len[h];
-                        const float x = s[nt][2 * h + e] * ((e ? k2.y : k2.x) * c_row[h]);
-                        s[nt][2 * h + e] = seen[h][nt][e] ? x : -INFINITY;
-                        mx[h] = fmaxf(mx[h], s[nt][2 * h + e]);
-                    }
+                    for (int r = 1; r < GR; r++) mx = fmaxf(mx, fmaxf(sc[r][n][e], sc[r][n][2 + e]));
+#pragma unroll
+                    for (int x = 4; x <= 16; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+                    const float mn = fmaxf(m[n][e], mx);
+                    top[n][e] = mn == -INFINITY ? 0.0f : mn;             // a row that has seen nothing yet
+                    f[n][e] = mn == m[n][e] ? 1.0f : ex2(m[n][e] - top[n][e]);
+                    m[n][e] = mn;
+                    moved = moved || f[n][e] != 1.0f;
                 }
-            }
-            vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, 1));
-            vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, 2));
-            const uint32_t r_new = max(r_bits, min((__float_as_uint(vmax) + 0x7FFFFFu) & 0x7F800000u, 253u << 23));
-            const float shrink = __uint_as_float(r_bits - r_new + (127u << 23));         // R / R', zero when that is below 2^-126
-            float f[2];
-#pragma unroll
-            for (int h = 0; h < HALVES; h++) {
-                mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
-                mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
-                const float mn = fmaxf(m[h], mx[h]);
-                mx[h] = mn == -INFINITY ? 0.0f : mn;     // a row that has seen nothing yet
-                f[h] = mn == m[h] ? 1.0f : ex2(m[h] - mx[h]);
-                m[h] = mn;
-            }
-            const bool moved = r_new != r_bits || f[0] != 1.0f || (HALVES == 2 && f[HALVES - 1] != 1.0f);
             if (__any_sync(0xffffffffu, moved)) {
-                const float sh = r_new - r_bits >= (127u << 23) ? 0.0f : shrink;
+                const float sh = r_new - r_bits >= (127u << 23) ? 0.0f : __uint_as_float(r_bits - r_new + (127u << 23));      // R / R'
 #pragma unroll
-                for (int c = 0; c < CH; c++)
+                for (int n = 0; n < NT; n++)
 #pragma unroll
-                    for (int x = 0; x < 2; x++)
+                    for (int e = 0; e < 2; e++) {
+                        l[n][e] *= f[n][e];
+                        const float x = f[n][e] * sh;
 #pragma unroll
-                        for (int h = 0; h < HALVES; h++) {
-                            o[c][x][2 * h] *= f[h] * sh;
-                            o[c][x][2 * h + 1] *= f[h] * sh;
-                        }
-#pragma unroll
-                for (int h = 0; h < HALVES; h++) l[h] *= f[h];
+                        for (int c = 0; c < CH; c++) { o[n][c][e] *= x; o[n][c][2 + e] *= x; }
+                    }
                 r_bits = r_new;
             }
             const float inv_r = __uint_as_float(((127u + 127u + 15u) << 23) - r_bits);   // 2^15 / R
-            uint32_t pa[TERMS][4];
+            uint32_t pb[TERMS][GR][NT][2];
 #pragma unroll
-            for (int x = 0; x < TERMS; x++) pa[x][1] = pa[x][3] = 0u;
+            for (int r = 0; r < GR; r++)
 #pragma unroll
-            for (int nt = 0; nt < 2; nt++)
+                for (int h = 0; h < 2; h++) {
+                    const float vr = vw[r][h] * inv_r;
 #pragma unroll
-                for (int h = 0; h < HALVES; h++) {
-                    float w[2];
+                    for (int n = 0; n < NT; n++) {
+                        float w[2];
 #pragma unroll
-                    for (int e = 0; e < 2; e++) {
-                        const float x = ex2(s[nt][2 * h + e] - mx[h]);
-                        l[h] += x;
-                        w[e] = seen[h][nt][e] ? x * (vw[nt][e] * inv_r) : 0.0f;
-                    }
-                    pa[0][h + 2 * nt] = pack_f16(w[0], w[1]);
-                    if (TERMS == 2) pa[TERMS - 1][h + 2 * nt] = pack_f16_rest(w[0], w[1], pa[0][h + 2 * nt]);
-                }
-            // ---- weighted values ----
-#pragma unroll
-            for (int c = 0; c < CH; c += 2) {
-                // matrices (positions 0-7, chunk c), (8-15, c), (0-7, c + 1), (8-15, c + 1)
-                const int row = (lane & 7) + 8 * (lane >> 3 & 1), ch = c + (lane >> 4);
-                uint32_t b[4];
-                ldmatrix_x4_trans(b, st + St::V + row * HD + 16 * (ch ^ (HD == 128 ? row & 7 : (row >> 1) & 3)));
-#pragma unroll
-                for (int x = 0; x < 2; x++) {
-                    const uint32_t lo = __byte_perm(b[2 * x], 0, 0x3120), hi = __byte_perm(b[2 * x + 1], 0, 0x3120);
-#pragma unroll
-                    for (int par = 0; par < 2; par++) {
-                        const uint32_t b0 = codes_to_f16(par ? lo >> 16 : lo & 0xFFFFu), b1 = codes_to_f16(par ? hi >> 16 : hi & 0xFFFFu);
-#pragma unroll
-                        for (int y = 0; y < TERMS; y++) mma_f16(o[c + x][par], pa[y], b0, b1);
+                        for (int e = 0; e < 2; e++) {
+                            const float x = ex2(sc[r][n][2 * h + e] - top[n][e]);
+                            l[n][e] += x;
+                            w[e] = x * vr;
+                            if (!all && sc[r][n][2 * h + e] == -INFINITY) w[e] = 0.0f;          // not 0 * NaN
+                        }
+                        const uint32_t hi = pack_f16(w[0], w[1]);
+                        pb[0][r][n][h] = transposed(hi);
+                        if (TERMS == 2) pb[TERMS - 1][r][n][h] = transposed(pack_f16_rest(w[0], w[1], hi));
                     }
                 }
-            }
+            // ---- weighted values: 16 dimensions a product ----
+#pragma unroll
+            for (int r = 0; r < GR; r++)
+#pragma unroll
+                for (int c = 0; c < CH; c += 2) {
+                    // matrices (positions 0-7, chunk c), (8-15, c), (0-7, c + 1), (8-15, c + 1)
+                    uint32_t b[4];
+                    ldmatrix_x4_trans(b, vt + r * HW * 16 * HD + chunk_at<HD>((lane & 7) + 8 * (lane >> 3 & 1), c + (lane >> 4)));
+#pragma unroll
+                    for (int x = 0; x < 2; x++) {
+                        uint32_t a[4];
+                        codes_to_f16(__byte_perm(b[2 * x], 0, 0x3120), a[0], a[1]);
+                        codes_to_f16(__byte_perm(b[2 * x + 1], 0, 0x3120), a[2], a[3]);
+#pragma unroll
+                        for (int n = 0; n < NT; n++)
+#pragma unroll
+                            for (int y = 0; y < TERMS; y++) mma_f16(o[n][c + x], a, pb[y][r][n][0], pb[y][r][n][1]);
+                    }
+                }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&empty[stage]);
+            if (++stage == NST) { stage = 0; phase ^= 1; }
         }
-        asm volatile("cp.async.wait_all;" ::: "memory");
-        __syncwarp();                                    // the ring may be filled again
         // ---- the row block's part is done: out, or into the workspace ----
         const float back = __uint_as_float(r_bits - (15u << 23));        // R / 2^15
-        const bool whole = t0 == 0 && t1 == tiles;
-        const int slot = blockIdx.x * 2 + (u == u_begin ? 0 : 1);
+        const bool whole = s.t0 == 0 && s.t1 == s.tiles;
+        const int slot = blockIdx.x * 2 + (s.first ? 0 : 1);
         float *ws_o = ws + (size_t)slot * HW * RB * HD;
         float2 *ws_ml = reinterpret_cast<float2 *>(ws + (size_t)gridDim.x * 2 * HW * RB * HD) + (size_t)slot * HW * RB;
 #pragma unroll
-        for (int h = 0; h < HALVES; h++) {
-            l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
-            l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
-        }
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int e = 0; e < 2; e++)
+#pragma unroll
+                for (int x = 4; x <= 16; x <<= 1) l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], x);
         if constexpr (PW == 1) {
 #pragma unroll
-            for (int h = 0; h < HALVES; h++) {
-                const int i = g + 8 * h;
-                if (i >= n_rows) continue;
-                const float norm = whole ? (l[h] == 0.0f ? 0.0f : back / l[h]) : back;
+            for (int n = 0; n < NT; n++)
 #pragma unroll
-                for (int c = 0; c < CH; c++) {
-                    const float4 v = make_float4(o[c][0][2 * h] * norm, o[c][1][2 * h] * norm, o[c][0][2 * h + 1] * norm, o[c][1][2 * h + 1] * norm);
-                    const int d = 16 * c + 4 * t;
-                    if (whole) store4(p.out, q_off[h] + d, v, bf16);
-                    else *reinterpret_cast<float4 *>(ws_o + ((size_t)(warp / PW) * RB + i) * HD + d) = v;
+                for (int e = 0; e < 2; e++) {
+                    const int i = 8 * n + 2 * t + e, rr = s.rb * RB + i;
+                    if (i >= s.n_rows) continue;
+                    const float norm = whole ? (l[n][e] == 0.0f ? 0.0f : back / l[n][e]) : back;
+                    const size_t off = ((size_t)(s.r.first + rr / group) * p.n_heads + (size_t)kvh * group + rr % group) * HD;
+#pragma unroll
+                    for (int c = 0; c < CH; c++) {
+                        const float2 v = make_float2(o[n][c][e] * norm, o[n][c][2 + e] * norm);
+                        if (whole) store2(p.out, off + 16 * c + 2 * g, v, bf16);
+                        else *reinterpret_cast<float2 *>(ws_o + ((size_t)hw * RB + i) * HD + 16 * c + 2 * g) = v;
+                    }
+                    if (!whole && g == 0) ws_ml[hw * RB + i] = make_float2(m[n][e], l[n][e]);
                 }
-                if (!whole && t == 0) ws_ml[(warp / PW) * RB + i] = make_float2(m[h], l[h]);
-            }
         } else {
-            // the PW warps of a head meet in shared memory: [warp][row][HD] and [warp][row] {maximum, sum}
-            float *po = reinterpret_cast<float *>(sh_smem);
-            float2 *pml = reinterpret_cast<float2 *>(po + SH_WARPS * RB * HD);
-            __syncthreads();                             // every warp has left its ring
+            // the PW warps of a head meet in shared memory, 16 PASS dimensions at a time
+            constexpr int D = 16 * PASS;
+            float2 *ml = reinterpret_cast<float2 *>(meet + SH_WARPS * RB * D);
 #pragma unroll
-            for (int h = 0; h < HALVES; h++) {
-                const int i = g + 8 * h;
+            for (int c0 = 0; c0 < CH; c0 += PASS) {
+                named_barrier_sync(1, SH_THREADS);       // what was there has been read
 #pragma unroll
-                for (int c = 0; c < CH; c++)
-                    *reinterpret_cast<float4 *>(po + ((size_t)warp * RB + i) * HD + 16 * c + 4 * t) =
-                        make_float4(o[c][0][2 * h] * back, o[c][1][2 * h] * back, o[c][0][2 * h + 1] * back, o[c][1][2 * h + 1] * back);
-                if (t == 0) pml[warp * RB + i] = make_float2(m[h], l[h]);
-            }
-            __syncthreads();
-            for (int x = tid; x < HW * n_rows * (HD / 4); x += SH_THREADS) {
-                const int d = 4 * (x % (HD / 4)), i = x / (HD / 4) % n_rows, hd = x / (HD / 4) / n_rows;
-                float mm = -INFINITY;
+                for (int n = 0; n < NT; n++)
 #pragma unroll
-                for (int w = 0; w < PW; w++) mm = fmaxf(mm, pml[(hd * PW + w) * RB + i].x);
-                const float base = mm == -INFINITY ? 0.0f : mm;
-                float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                float ll = 0.0f;
+                    for (int e = 0; e < 2; e++) {
+                        const int i = 8 * n + 2 * t + e;
 #pragma unroll
-                for (int w = 0; w < PW; w++) {
-                    const float2 ml = pml[(hd * PW + w) * RB + i];
-                    const float wt = ex2(ml.x - base);
-                    const float4 v = *reinterpret_cast<const float4 *>(po + ((size_t)(hd * PW + w) * RB + i) * HD + d);
-                    ll = fmaf(ml.y, wt, ll);
-                    a.x = fmaf(v.x, wt, a.x); a.y = fmaf(v.y, wt, a.y); a.z = fmaf(v.z, wt, a.z); a.w = fmaf(v.w, wt, a.w);
+                        for (int c = 0; c < PASS; c++)
+                            *reinterpret_cast<float2 *>(meet + ((size_t)warp * RB + i) * D + 16 * c + 2 * g) =
+                                make_float2(o[n][c0 + c][e] * back, o[n][c0 + c][2 + e] * back);
+                        if (g == 0) ml[warp * RB + i] = make_float2(m[n][e], l[n][e]);
+                    }
+                named_barrier_sync(1, SH_THREADS);
+                for (int x = tid; x < HW * s.n_rows * (D / 4); x += SH_THREADS) {
+                    const int d = 4 * (x % (D / 4)), i = x / (D / 4) % s.n_rows, hd = x / (D / 4) / s.n_rows;
+                    float mm = -INFINITY;
+#pragma unroll
+                    for (int w = 0; w < PW; w++) mm = fmaxf(mm, ml[(w * HW + hd) * RB + i].x);
+                    const float base = mm == -INFINITY ? 0.0f : mm;
+                    float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    float ll = 0.0f;
+#pragma unroll
+                    for (int w = 0; w < PW; w++) {
+                        const float2 v2 = ml[(w * HW + hd) * RB + i];
+                        const float wt = ex2(v2.x - base);
+                        const float4 v = *reinterpret_cast<const float4 *>(meet + ((size_t)(w * HW + hd) * RB + i) * D + d);
+                        ll = fmaf(v2.y, wt, ll);
+                        a.x = fmaf(v.x, wt, a.x); a.y = fmaf(v.y, wt, a.y); a.z = fmaf(v.z, wt, a.z); a.w = fmaf(v.w, wt, a.w);
+                    }
+                    if (whole) {
+                        const float norm = ll == 0.0f ? 0.0f : 1.0f / ll;
+                        const int rr = s.rb * RB + i;
+                        const size_t off = ((size_t)(s.r.first + rr / group) * p.n_heads + (size_t)(hg * HW + hd) * group + rr % group) * HD;
+                        store4(p.out, off + 16 * c0 + d, make_float4(a.x * norm, a.y * norm, a.z * norm, a.w * norm), bf16);
+                    } else {
+                        *reinterpret_cast<float4 *>(ws_o + ((size_t)hd * RB + i) * HD + 16 * c0 + d) = a;
+                        if (c0 == 0 && d == 0) ws_ml[hd * RB + i] = make_float2(mm, ll);
+                    }
                 }
-                if (whole) {
-                    const float norm = ll == 0.0f ? 0.0f : 1.0f / ll;
-                    const int rr = rb * RB + i;
-                    const size_t off = ((size_t)(r.first + rr / group) * p.n_heads + (size_t)(hg * HW + hd) * group + rr % group) * HD + d;
-                    store4(p.out, off, make_float4(a.x * norm, a.y * norm, a.z * norm, a.w * norm), bf16);
-                } else {
-                    *reinterpret_cast<float4 *>(ws_o + ((size_t)hd * RB + i) * HD + d) = a;
-                    if (d == 0) ws_ml[hd * RB + i] = make_float2(mm, ll);
-                }
             }
-            __syncthreads();                             // the ring may be filled again
         }
-        u += t1 - t0;
     }
 }
 
@@ -651,15 +814,14 @@ attention_quant_merge_kernel(const AttnQuant p, int bf16, const Rows rows, int c
     store4(p.out, ((size_t)gq * p.n_heads + head) * HD + d, make_float4(acc.x * norm, acc.y * norm, acc.z * norm, acc.w * norm), bf16);
 }
 
-struct ShortPlan { int rb, terms, hw, stages, per_sm; };
+struct ShortPlan { int rb, terms, hw, per_sm; };
 ShortPlan short_plan(const AttnQuant &p, int dtype) {
     const int group = p.n_heads / p.n_kv;
     ShortPlan s;
     s.rb = group <= 8 && p.total_q <= p.num_req ? 8 : 16;
     s.terms = dtype == DT_F32 ? 2 : 1;
-    s.hw = p.n_kv % 8 == 0 ? 8 : p.n_kv % 4 == 0 ? 4 : p.n_kv % 2 == 0 ? 2 : 1;
-    s.per_sm = s.rb == 8 && s.terms == 1 ? 2 : 1;
-    s.stages = s.per_sm == 2 ? 3 : 6;
+    s.hw = p.n_kv % 4 == 0 ? 4 : p.n_kv % 2 == 0 ? 2 : 1;
+    s.per_sm = 2;
     return s;
 }
 int short_grid(const AttnQuant &p, const ShortPlan &s, int sm_count) {
@@ -670,37 +832,67 @@ size_t short_workspace(const AttnQuant &p, const ShortPlan &s, int sm_count) {
     return (size_t)short_grid(p, s, sm_count) * 2 * s.hw * s.rb * (p.head_dim + 2) * sizeof(float);
 }
 
-template <int HD, int RB, int TERMS, int HW, int NST>
-cudaError_t launch_short(const AttnQuant &p, int dtype, int grid, int only_short, float *ws, cudaStream_t s, bool pdl) {
-    constexpr size_t ring = (size_t)SH_WARPS * NST * ShortStage<HD>::BYTES;
-    constexpr size_t meet = HW == SH_WARPS ? 0 : (size_t)SH_WARPS * RB * (HD + 2) * sizeof(float);
-    constexpr size_t smem = ring > meet ? ring : meet;
-    auto k = attention_quant_short_kernel<HD, RB, TERMS, HW, NST>;
+// What the launches of one call share.
+struct ShortCall {
+    ShortMaps maps;
+    int dtype, grid, only_short;
+    uint32_t polls;
+    float *ws;
+    bool tma, pdl;
+    cudaStream_t stream;
+};
+// Runs of 16 positions stay within a page, and the scales of a KV head start on 16 bytes.
+bool tma_fits(const AttnQuant &p) { return p.block_size % 16 == 0 && p.num_slots % 4 == 0; }
+
+cudaError_t encode_maps(const AttnQuant &p, int hw, ShortMaps *m) {
+    EncodeTiledFn enc = encode_tiled_fn();
+    if (!enc) return cudaErrorNotSupported;
+    const cuuint64_t dims[3] = {(cuuint64_t)p.head_dim, p.num_slots, (cuuint64_t)p.n_kv};
+    const cuuint64_t strides[2] = {(cuuint64_t)p.n_kv * p.head_dim, (cuuint64_t)p.head_dim};
+    const cuuint32_t box[3] = {(cuuint32_t)p.head_dim, 16, (cuuint32_t)hw}, step[3] = {1, 1, 1};
+    for (int i = 0; i < 2; i++) {
+        const CUresult r = enc(i ? &m->v : &m->k, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<uint8_t *>(i ? p.v_pool : p.k_pool), dims,
+                               strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                               p.head_dim == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                               CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+        if (r != CUDA_SUCCESS) return cudaErrorInvalidValue;
+        const cudaError_t e = encode_2d(i ? &m->vs : &m->ks, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, i ? p.v_scales : p.k_scales, p.num_slots,
+                                        (uint64_t)p.n_kv, (uint64_t)p.num_slots * 4, 16, (uint32_t)hw, CU_TENSOR_MAP_SWIZZLE_NONE);
+        if (e != cudaSuccess) return e;
+    }
+    return cudaSuccess;
+}
+
+template <int HD, int RB, int TERMS, int HW, int NST, bool TMA>
+cudaError_t launch_short(const AttnQuant &p, const ShortCall &c) {
+    constexpr size_t meet = HW == SH_WARPS ? 0 : (size_t)SH_WARPS * RB * (16 + 2) * sizeof(float);
+    using St = ShortStage<HD, HW>;
+    constexpr size_t smem = NST * (St::BYTES + St::AUX) + meet;
+    static_assert(2 * (smem + 2048) <= 228 * 1024, "two CTAs' shared memory");
+    auto k = attention_quant_short_kernel<HD, RB, TERMS, HW, NST, TMA>;
     const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;
-    return launch_dependent(k, dim3((unsigned)grid), dim3(SH_THREADS), smem, s, pdl, p, (int)(dtype == DT_BF16), only_short, ws);
+    return launch_dependent(k, dim3((unsigned)c.grid), dim3(SH_THREADS + (TMA ? 32 : 128)), smem, c.stream, c.pdl, c.maps, p,
+                            (int)(c.dtype == DT_BF16), c.only_short, c.polls, c.ws);
 }
 template <int HD, int RB, int TERMS, int NST>
-cudaError_t launch_short_hw(const AttnQuant &p, int dtype, int hw, int grid, int only_short, float *ws, cudaStream_t s, bool pdl) {
+cudaError_t launch_short_hw(const AttnQuant &p, int hw, const ShortCall &c) {
     switch (hw) {
-        case 8: return launch_short<HD, RB, TERMS, 8, NST>(p, dtype, grid, only_short, ws, s, pdl);
-        case 4: return launch_short<HD, RB, TERMS, 4, NST>(p, dtype, grid, only_short, ws, s, pdl);
-        case 2: return launch_short<HD, RB, TERMS, 2, NST>(p, dtype, grid, only_short, ws, s, pdl);
-        default: return launch_short<HD, RB, TERMS, 1, NST>(p, dtype, grid, only_short, ws, s, pdl);
+        case 4: return c.tma ? launch_short<HD, RB, TERMS, 4, NST, true>(p, c) : launch_short<HD, RB, TERMS, 4, NST, false>(p, c);
+        case 2: return c.tma ? launch_short<HD, RB, TERMS, 2, NST, true>(p, c) : launch_short<HD, RB, TERMS, 2, NST, false>(p, c);
+        default: return c.tma ? launch_short<HD, RB, TERMS, 1, NST, true>(p, c) : launch_short<HD, RB, TERMS, 1, NST, false>(p, c);
     }
 }
 template <int HD>
-cudaError_t launch_short_all(const AttnQuant &p, int dtype, const ShortPlan &pl, int sm_count, int only_short, float *ws, cudaStream_t s, bool pdl) {
-    const int grid = short_grid(p, pl, sm_count);
+cudaError_t launch_short_all(const AttnQuant &p, const ShortPlan &pl, const ShortCall &c) {
     cudaError_t e;
-    if (pl.terms == 2) e = pl.rb == 8 ? launch_short_hw<HD, 8, 2, 6>(p, dtype, pl.hw, grid, only_short, ws, s, pdl)
-                                      : launch_short_hw<HD, 16, 2, 6>(p, dtype, pl.hw, grid, only_short, ws, s, pdl);
-    else e = pl.rb == 8 ? launch_short_hw<HD, 8, 1, 3>(p, dtype, pl.hw, grid, only_short, ws, s, pdl)
-                        : launch_short_hw<HD, 16, 1, 6>(p, dtype, pl.hw, grid, only_short, ws, s, pdl);
+    constexpr int NST = HD == 128 ? 3 : 5;
+    if (pl.terms == 2) e = pl.rb == 8 ? launch_short_hw<HD, 8, 2, NST>(p, pl.hw, c) : launch_short_hw<HD, 16, 2, NST>(p, pl.hw, c);
+    else e = pl.rb == 8 ? launch_short_hw<HD, 8, 1, NST>(p, pl.hw, c) : launch_short_hw<HD, 16, 1, NST>(p, pl.hw, c);
     if (e != cudaSuccess) return e;
-    const Rows rows{pl.rb, 16 * SH_WARPS / pl.hw, pl.hw, only_short};
-    return launch_dependent(attention_quant_merge_kernel<HD>, dim3((unsigned)p.total_q * p.n_heads), dim3(MERGE_THREADS), 0, s, pdl,
-                            p, (int)(dtype == DT_BF16), rows, grid / (p.n_kv / pl.hw), (const float *)ws);
+    const Rows rows{pl.rb, 16 * SH_TILES / pl.hw, pl.hw, c.only_short};
+    return launch_dependent(attention_quant_merge_kernel<HD>, dim3((unsigned)p.total_q * p.n_heads), dim3(MERGE_THREADS), 0, c.stream, c.pdl,
+                            p, (int)(c.dtype == DT_BF16), rows, c.grid / (p.n_kv / pl.hw), (const float *)c.ws);
 }
 
 bool mma_supported(const AttnQuant &p) { return p.head_dim == 64 || p.head_dim == 128; }
@@ -711,8 +903,8 @@ size_t attention_quant_workspace(const AttnQuant &p, int dtype, int sm_count) {
     return mma_supported(p) ? short_workspace(p, short_plan(p, dtype), sm_count) : 0;
 }
 
-cudaError_t launch_attention_quant(const AttnQuant &p, int dtype, float *ws, int sm_count, cudaStream_t s, bool pdl,
-                                   uint64_t *launches) {
+cudaError_t launch_attention_quant(const AttnQuant &p, int dtype, float *ws, int sm_count, uint32_t polls, cudaStream_t s,
+                                   bool pdl, uint64_t *launches) {
     if (p.total_q <= 0 || p.num_req <= 0) return cudaSuccess;
     if (!mma_supported(p)) {
         ++*launches;
@@ -720,9 +912,15 @@ cudaError_t launch_attention_quant(const AttnQuant &p, int dtype, float *ws, int
                                 (int)(dtype == DT_BF16));
     }
     const ShortPlan pl = short_plan(p, dtype);
+    ShortCall c = {};
+    c.dtype = dtype; c.grid = short_grid(p, pl, sm_count); c.polls = polls; c.ws = ws; c.pdl = pdl; c.stream = s;
+    c.tma = tma_fits(p);
+    if (c.tma) {
+        const cudaError_t e = encode_maps(p, pl.hw, &c.maps);
+        if (e != cudaSuccess) return e;
+    }
     *launches += 2;
-    return p.head_dim == 128 ? launch_short_all<128>(p, dtype, pl, sm_count, 0, ws, s, pdl)
-                             : launch_short_all<64>(p, dtype, pl, sm_count, 0, ws, s, pdl);
+    return p.head_dim == 128 ? launch_short_all<128>(p, pl, c) : launch_short_all<64>(p, pl, c);
 }
 
 }  // namespace llmrs

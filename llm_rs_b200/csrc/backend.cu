@@ -1333,7 +1333,7 @@ int llmrs_cuda_attention_quant(llmrs_ctx *ctx, llmrs_buf *out, const llmrs_buf *
     e = ctx->begin_work();
     PerfScope perf(ctx, name, 2.0 * buf_elems(q) * dense_elem_bytes(q->dtype), 0.0);    // q and out: the lengths live on the device
     if (e == cudaSuccess)
-        e = launch_attention_quant(p, (int)q->dtype, ctx->att_ws, ctx->sm_count, ctx->stream, ctx->pdl, &ctx->launches);
+        e = launch_attention_quant(p, (int)q->dtype, ctx->att_ws, ctx->sm_count, ctx->mbar_polls, ctx->stream, ctx->pdl, &ctx->launches);
     if (e != cudaSuccess) return ctx->cuda_fail(e, name);
     return LLMRS_OK;
 }

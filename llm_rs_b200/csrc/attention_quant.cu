@@ -153,7 +153,9 @@ __global__ void __launch_bounds__(AQ_TILE) attention_quant_simple_kernel(const A
 // row block's next 16 PW positions, PW = 8 / HW, for HW KV heads at once.  The units of all requests form one
 // sequence that is cut into equal contiguous ranges, one per CTA, so ragged batches load every SM alike and one
 // long request spreads over the whole GPU.  The lengths are on the device, so each CTA adds them up itself.  A row
-// block that lies in several ranges leaves (accumulator, maximum, sum) in the workspace for the merge kernel.
+// block that lies in several ranges leaves (accumulator, maximum, sum) parts in the workspace; the last CTA to finish of
+// each 18 neighbours joins theirs, and the last of those the rest, always in the order of the parts (a second
+// kernel for it cost 5 us of 14 for one request of 1000 positions and 65 us beside 97 for 64 requests).
 //
 // A CTA has 8 consumer warps, HW heads x PW runs of 16 positions, so that neighbouring heads of a slot, neighbours
 // in memory, are read at the same time, and a producer that keeps NST units in flight, through to the end of the
@@ -191,51 +193,64 @@ __device__ __forceinline__ void shape_of(const AttnQuant &p, const Rows &w, cons
     const int len = r.before + r.count;
     tiles = len > 0 ? (int)(((long long)len + w.tp - 1) / w.tp) : 1;     // a row block that sees nothing still writes its zeros
 }
-// All threads of the CTA: the units of all requests (returned), and into found[] the request that holds unit
-// `want(total)` and the units before that request; or, with `req` >= 0, the units before that request.
+// A whole warp, every warp for itself: the units of all requests (returned), and the request that holds unit
+// want(total), its data and the units before it.
+struct Found {
+    int req;
+    Request r;
+    long long before;
+};
 template <typename Want>
-__device__ __forceinline__ long long scan_units(const AttnQuant &p, const Rows &w, long long *sums, long long *found, Want want, int req) {
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
-    auto units = [&](int r) -> long long {
-        if (r >= p.num_req) return 0;
+__device__ __forceinline__ long long scan_units(const AttnQuant &p, const Rows &w, Want want, Found &found) {
+    const int lane = threadIdx.x & 31;
+    auto units = [&](int req, Request &r) -> long long {
+        if (req >= p.num_req) return 0;
         int b, t;
-        shape_of(p, w, request_of(p, r), b, t);
+        r = request_of(p, req);
+        shape_of(p, w, r, b, t);
         return (long long)b * t;
     };
-    const long long mine = units(tid);                   // the first blockDim.x requests stay in registers
-    long long s = mine;
-    for (int r = tid + blockDim.x; r < p.num_req; r += blockDim.x) s += units(r);
+    Request r0 = {0, 0, 0};
+    const long long u0 = units(lane, r0);                // the first 32 requests stay in registers
+    long long total = u0;
+#pragma unroll 4
+    for (int q = lane + 32; q < p.num_req; q += 32) {
+        Request r;
+        total += units(q, r);
+    }
 #pragma unroll
-    for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    if (lane == 0) sums[warp] = s;
-    __syncthreads();
-    long long total = 0;
-    for (int i = 0; i < warps; i++) total += sums[i];
-    __syncthreads();
+    for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
     const long long at = want(total);
+    if (at < 0 || total == 0) return total;
     long long base = 0;
-    for (int r0 = 0; r0 < p.num_req; r0 += blockDim.x) {
-        const long long u = r0 == 0 ? mine : units(r0 + tid);
+    for (int q0 = 0; q0 < p.num_req; q0 += 32) {
+        Request r = r0;
+        const long long u = q0 == 0 ? u0 : units(q0 + lane, r);
         long long inc = u;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const long long v = __shfl_up_sync(0xffffffffu, inc, o);
             if (lane >= o) inc += v;
         }
-        if (lane == 31) sums[warp] = inc;
-        __syncthreads();
-        long long before = base + inc - u;
-        for (int i = 0; i < warp; i++) before += sums[i];
-        if (req >= 0 ? r0 + tid == req : (u > 0 && at >= before && at < before + u)) { found[0] = r0 + tid; found[1] = before; }
-        for (int i = 0; i < warps; i++) base += sums[i];
-        __syncthreads();
+        const unsigned hit = __ballot_sync(0xffffffffu, at < base + inc);       // the first of them holds it: empty ones have inc as before
+        if (hit) {
+            const int src = __ffs(hit) - 1;
+            found.req = q0 + src;
+            found.r.first = __shfl_sync(0xffffffffu, r.first, src);
+            found.r.count = __shfl_sync(0xffffffffu, r.count, src);
+            found.r.before = __shfl_sync(0xffffffffu, r.before, src);
+            found.before = base + __shfl_sync(0xffffffffu, inc - u, src);
+            return total;
+        }
+        base += __shfl_sync(0xffffffffu, inc, 31);
     }
     return total;
 }
+constexpr int SH_JOIN = 18;          // parts that are joined at once: two levels reach two CTAs on each of 148 SMs
 // CTAs (per head group) that share `total` units, and the range of one; the CTA that holds unit u.
 __device__ __forceinline__ int sharers(long long total, int ctas) {
     const long long most = (total + SH_MIN_UNITS - 1) / SH_MIN_UNITS;
-    return (int)min((long long)ctas, max(most, 1ll));
+    return (int)min((long long)min(ctas, SH_JOIN * (SH_JOIN - 1)), max(most, 1ll));      // what two levels of joining reach
 }
 __device__ __forceinline__ long long first_unit(long long total, int n, int c) { return total * c / n; }
 __device__ __forceinline__ int holder(long long total, int n, long long u) { return (int)(((u + 1) * n - 1) / total); }
@@ -305,17 +320,23 @@ template <int HD> __device__ __forceinline__ int chunk_at(int row, int c) {
 struct Segment {
     Request r;
     int req, rb, t0, t1, tiles, n_rows, kv_end, n_steps;
+    long long item;                  // the row block's first unit
     bool first;                      // starts where the range starts
 };
 template <int RB, int TP> struct Walk {
     long long u, u_begin, u_end, req_base;
     int req;
+    Request r;                       // of `req`
     __device__ __forceinline__ bool next(const AttnQuant &p, const Rows &w, Segment &s) {
         while (u < u_end) {
             int blocks;
-            s.r = request_of(p, req);
-            shape_of(p, w, s.r, blocks, s.tiles);
-            if (u >= req_base + (long long)blocks * s.tiles) { req_base += (long long)blocks * s.tiles; req++; continue; }
+            shape_of(p, w, r, blocks, s.tiles);
+            if (u >= req_base + (long long)blocks * s.tiles) {
+                req_base += (long long)blocks * s.tiles;
+                r = request_of(p, ++req);
+                continue;
+            }
+            s.r = r;
             const int group = p.n_heads / p.n_kv;
             s.req = req;
             s.rb = (int)((u - req_base) / s.tiles);
@@ -325,6 +346,7 @@ template <int RB, int TP> struct Walk {
             s.kv_end = s.r.before + (s.rb * RB + s.n_rows - 1) / group + 1;
             s.n_steps = max(0, min(s.t1, (max(s.kv_end, 0) + TP - 1) / TP) - s.t0);   // 0: nothing to see in this range
             s.first = u == u_begin;
+            s.item = u - s.t0;
             u += s.t1 - s.t0;
             return true;
         }
@@ -332,18 +354,103 @@ template <int RB, int TP> struct Walk {
     }
 };
 
+// Where a row block's parts are, CTAs c0 .. c1 of head group hg.
+struct Parts {
+    long long total, item;
+    int n_cta, groups, hg;
+    __device__ __forceinline__ int slot(int c) const {   // of CTA c: its first part, or its second if the row block starts within its range
+        const long long f = first_unit(total, n_cta, c);
+        return (c * groups + hg) * 2 + (item > f ? 1 : 0);
+    }
+};
+// The consumer threads of a CTA: joins n <= SH_JOIN parts of HW heads x n_rows rows, part i in workspace slot slots(i); into
+// the output (`last`) or into the first of the slots.
+template <int HD, int RB, int HW, typename Slots>
+__device__ __forceinline__ void join_parts(const AttnQuant &p, int bf16, const Segment &s, int hg, float *ws, float2 *ws_ml, float2 *ml_s, int *slot_s,
+                                           int n, bool last, Slots slots) {
+    const int tid = threadIdx.x, rows = HW * s.n_rows, group = p.n_heads / p.n_kv;
+    if (tid < n) slot_s[tid] = slots(tid);               // a division of 64 bits each: once
+    named_barrier_sync(1, SH_THREADS);
+    for (int x = tid; x < n * rows; x += SH_THREADS) {
+        const int i = x / rows, r = x - i * rows;
+        ml_s[x] = __ldcg(ws_ml + (size_t)slot_s[i] * HW * RB + r / s.n_rows * RB + r % s.n_rows);
+    }
+    named_barrier_sync(1, SH_THREADS);
+    // Four elements (16 bytes) of the result a thread at a time, four parts of each: 16 loads under way.
+    constexpr int E = 4;
+    for (int x0 = tid; x0 < rows * (HD / 4); x0 += E * SH_THREADS) {
+        int r[E];
+        size_t at[E];
+        float m[E], l[E];
+        float4 a[E];
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+            const int x = min(x0 + e * SH_THREADS, rows * (HD / 4) - 1);         // past the end: the last one again, not stored
+            r[e] = x / (HD / 4);
+            at[e] = ((size_t)(r[e] / s.n_rows) * RB + r[e] % s.n_rows) * HD + 4 * (x % (HD / 4));
+            m[e] = -INFINITY;
+            for (int y = 0; y < n; y++) m[e] = fmaxf(m[e], ml_s[y * rows + r[e]].x);
+            l[e] = 0.0f;
+            a[e] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        }
+#pragma unroll 4
+        for (int y = 0; y < n; y++) {
+            const float *part = ws + (size_t)slot_s[y] * HW * RB * HD;
+#pragma unroll
+            for (int e = 0; e < E; e++) {
+                const float4 v = __ldcg(reinterpret_cast<const float4 *>(part + at[e]));
+                const float2 ml = ml_s[y * rows + r[e]];
+                const float w = ex2(ml.x - (m[e] == -INFINITY ? 0.0f : m[e]));
+                l[e] = fmaf(ml.y, w, l[e]);
+                a[e].x = fmaf(v.x, w, a[e].x); a[e].y = fmaf(v.y, w, a[e].y); a[e].z = fmaf(v.z, w, a[e].z); a[e].w = fmaf(v.w, w, a[e].w);
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+            const int x = x0 + e * SH_THREADS;
+            if (x >= rows * (HD / 4)) break;
+            const int d = 4 * (x % (HD / 4)), i = r[e] % s.n_rows, hd = r[e] / s.n_rows;
+            if (last) {
+                const float norm = l[e] == 0.0f ? 0.0f : 1.0f / l[e];
+                const int rr = s.rb * RB + i;
+                store4(p.out, ((size_t)(s.r.first + rr / group) * p.n_heads + (size_t)(hg * HW + hd) * group + rr % group) * HD + d,
+                       make_float4(a[e].x * norm, a[e].y * norm, a[e].z * norm, a[e].w * norm), bf16);
+            } else {                                     // this thread alone has read what it overwrites; the pairs were copied
+                const size_t to = ((size_t)slot_s[0] * HW + hd) * RB + i;
+                *reinterpret_cast<float4 *>(ws + to * HD + d) = a[e];
+                if (d == 0) ws_ml[to] = make_float2(m[e], l[e]);
+            }
+        }
+    }
+}
+// Counts this CTA in; true in the one that completes `n`, which also clears the counter for the next launch.
+__device__ __forceinline__ bool last_of(uint32_t *counter, uint32_t n, uint32_t *flag) {
+    __threadfence();                                     // this thread's part is visible before the CTA is counted
+    named_barrier_sync(1, SH_THREADS);
+    if (threadIdx.x == 0) {
+        const bool l = atomicAdd(counter, 1u) == n - 1;
+        if (l) *counter = 0;
+        *flag = l;
+        __threadfence();
+    }
+    named_barrier_sync(1, SH_THREADS);
+    return *flag != 0;
+}
+
 template <int HD, int RB, int TERMS, int HW, int NST, bool TMA>
 __global__ void __launch_bounds__(SH_THREADS + (TMA ? 32 : 128), 2)
 attention_quant_short_kernel(const __grid_constant__ ShortMaps maps, const AttnQuant p, int bf16, int only_short, uint32_t polls,
-                             float *__restrict__ ws) {
+                             float *__restrict__ ws, uint32_t *__restrict__ counters) {
     using St = ShortStage<HD, HW>;
     constexpr int PW = SH_WARPS / HW, RUNS = St::RUNS, TP = 16 * RUNS, KS = HD / 16, CH = HD / 16, NT = RB / 8;
     constexpr int PASS = 1;                              // chunks of 16 dimensions the warps of a head exchange at a time
     extern __shared__ __align__(1024) uint8_t sh_smem[];
     uint8_t *codes = sh_smem, *aux = codes + NST * St::BYTES;
-    float *meet = reinterpret_cast<float *>(aux + NST * St::AUX);            // PW > 1: [warp][row][16 PASS] and [warp][row] {max, sum}
+    float2 *join = reinterpret_cast<float2 *>(aux + NST * St::AUX);          // {max, sum} of the rows of up to SH_JOIN parts
+    float *meet = reinterpret_cast<float *>(join + SH_JOIN * HW * RB);       // PW > 1: [warp][row][16 PASS] and [warp][row] {max, sum}
+    __shared__ uint32_t is_last;
+    __shared__ int slot_s[SH_JOIN];
     __shared__ __align__(8) uint64_t full[NST], empty[NST];
-    __shared__ long long sums[(SH_THREADS + (TMA ? 32 : 128)) / 32], found[2];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     if (tid == 0) {
         for (int i = 0; i < NST; i++) {
@@ -352,21 +459,24 @@ attention_quant_short_kernel(const __grid_constant__ ShortMaps maps, const AttnQ
         }
         mbar_init_fence();
     }
+    __syncthreads();
     pdl_prologue();
     const int groups = p.n_kv / HW, hg = blockIdx.x % groups, cta = blockIdx.x / groups, ctas = gridDim.x / groups;
     const int group = p.n_heads / p.n_kv;
     const Rows rows{RB, TP, HW, only_short};
     int n_cta = 1;
-    const long long total = scan_units(p, rows, sums, found, [&](long long all) {
+    Found found;
+    const long long total = scan_units(p, rows, [&](long long all) {
         n_cta = sharers(all, ctas);
         return cta < n_cta ? first_unit(all, n_cta, cta) : -1ll;
-    }, -1);                                              // its barriers also publish the mbarriers
-    if (cta >= n_cta || total == 0) return;
+    }, found);
+    if (cta >= n_cta || total == 0) return;              // the same for every warp
     Walk<RB, TP> walk;
     walk.u = walk.u_begin = first_unit(total, n_cta, cta);
     walk.u_end = first_unit(total, n_cta, cta + 1);
-    walk.req = (int)found[0];
-    walk.req_base = found[1];
+    walk.req = found.req;
+    walk.req_base = found.before;
+    walk.r = found.r;
     Segment s;
     int stage = 0;
     uint32_t phase = 0;
@@ -739,79 +849,20 @@ attention_quant_short_kernel(const __grid_constant__ ShortMaps maps, const AttnQ
                 }
             }
         }
+        if (whole) continue;
+        const Parts parts{total, s.item, n_cta, groups, hg};
+        const int c0 = holder(total, n_cta, s.item), c1 = holder(total, n_cta, s.item + s.tiles - 1);
+        const int g0 = cta / SH_JOIN * SH_JOIN, gf = max(c0, g0), gl = min(c1, g0 + SH_JOIN - 1);    // of these neighbours
+        const bool near = gf == c0 && gl == c1;
+        float2 *all_ml = reinterpret_cast<float2 *>(ws + (size_t)gridDim.x * 2 * HW * RB * HD);
+        if (!last_of(counters + parts.slot(gf), (uint32_t)(gl - gf + 1), &is_last)) continue;
+        join_parts<HD, RB, HW>(p, bf16, s, hg, ws, all_ml, join, slot_s, gl - gf + 1, near, [&](int i) { return parts.slot(gf + i); });
+        if (near) continue;
+        const int n_far = c1 / SH_JOIN - c0 / SH_JOIN + 1;
+        if (!last_of(counters + gridDim.x * 2 + parts.slot(c0), (uint32_t)n_far, &is_last)) continue;
+        join_parts<HD, RB, HW>(p, bf16, s, hg, ws, all_ml, join, slot_s, n_far, true,
+                               [&](int i) { return parts.slot(max(c0, (c0 / SH_JOIN + i) * SH_JOIN)); });
     }
-}
-
-// One CTA per (query token, head): the parts of its row, if they were left by several CTAs, joined in order.  A
-// quarter (head_dim 64: an eighth) of a warp's lanes would do for a part; HD / 4 threads take one each round.
-constexpr int MERGE_THREADS = 512;
-template <int HD>
-__global__ void __launch_bounds__(MERGE_THREADS)
-attention_quant_merge_kernel(const AttnQuant p, int bf16, const Rows rows, int ctas, const float *__restrict__ ws) {
-    pdl_prologue();
-    constexpr int PER = MERGE_THREADS / (HD / 4);        // parts at a time
-    __shared__ long long sums[MERGE_THREADS / 32], found[2];
-    __shared__ float4 acc_s[MERGE_THREADS];
-    __shared__ float red[MERGE_THREADS / 32], lsum[PER];
-    const int head = blockIdx.x % p.n_heads, gq = blockIdx.x / p.n_heads, tid = threadIdx.x;
-    const int group = p.n_heads / p.n_kv, kvh = head / group;
-    int req = 0;
-    Request r;
-    for (; req < p.num_req; req++) {
-        r = request_of(p, req);
-        if (gq >= r.first && gq < r.first + r.count) break;
-    }
-    if (req == p.num_req) return;
-    const long long total = scan_units(p, rows, sums, found, [](long long) { return 0ll; }, req);
-    int blocks, tiles;
-    shape_of(p, rows, r, blocks, tiles);
-    if (blocks == 0) return;                             // the other kernel's
-    const int rr = (gq - r.first) * group + head % group, rb = rr / rows.rb, i = rr % rows.rb;
-    const int n = sharers(total, ctas), groups = p.n_kv / rows.hw, hg = kvh / rows.hw, hd = kvh % rows.hw;
-    const long long a = found[1] + (long long)rb * tiles;
-    const int c0 = holder(total, n, a), c1 = holder(total, n, a + tiles - 1);
-    if (c0 == c1) return;                                // one CTA had all of it and wrote the row
-    const size_t slots = (size_t)ctas * groups * 2;
-    const float2 *ml = reinterpret_cast<const float2 *>(ws + slots * rows.hw * rows.rb * HD);
-    auto part = [&](int c) {                             // index of CTA c's part of this row
-        const int which = max(a, first_unit(total, n, c)) == first_unit(total, n, c) ? 0 : 1;
-        return ((size_t)((c * groups + hg) * 2 + which) * rows.hw + hd) * rows.rb + i;
-    };
-    float m = -INFINITY;
-    for (int c = c0 + tid; c <= c1; c += MERGE_THREADS) m = fmaxf(m, ml[part(c)].x);
-#pragma unroll
-    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    if ((tid & 31) == 0) red[tid >> 5] = m;
-    __syncthreads();
-    m = red[0];
-    for (int w = 1; w < MERGE_THREADS / 32; w++) m = fmaxf(m, red[w]);
-    const float base = m == -INFINITY ? 0.0f : m;
-    const int d = 4 * (tid % (HD / 4)), lane_part = tid / (HD / 4);
-    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    float l = 0.0f;
-#pragma unroll 4
-    for (int c = c0 + lane_part; c <= c1; c += PER) {
-        const size_t x = part(c);
-        const float2 v = ml[x];
-        const float4 q = *reinterpret_cast<const float4 *>(ws + x * HD + d);
-        const float w = ex2(v.x - base);
-        l = fmaf(v.y, w, l);
-        acc.x = fmaf(q.x, w, acc.x); acc.y = fmaf(q.y, w, acc.y); acc.z = fmaf(q.z, w, acc.z); acc.w = fmaf(q.w, w, acc.w);
-    }
-    acc_s[tid] = acc;
-    if (d == 0) lsum[lane_part] = l;
-    __syncthreads();
-    if (tid >= HD / 4) return;
-    float ll = 0.0f;
-    acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-    for (int x = 0; x < PER; x++) {
-        const float4 q = acc_s[x * (HD / 4) + tid];
-        ll += lsum[x];
-        acc.x += q.x; acc.y += q.y; acc.z += q.z; acc.w += q.w;
-    }
-    const float norm = ll == 0.0f ? 0.0f : 1.0f / ll;
-    store4(p.out, ((size_t)gq * p.n_heads + head) * HD + d, make_float4(acc.x * norm, acc.y * norm, acc.z * norm, acc.w * norm), bf16);
 }
 
 struct ShortPlan { int rb, terms, hw, per_sm; };
@@ -824,6 +875,7 @@ ShortPlan short_plan(const AttnQuant &p, int dtype) {
     s.per_sm = 2;
     return s;
 }
+constexpr int SHORT_MAX_GROUPS = 2048;       // head groups of a call
 int short_grid(const AttnQuant &p, const ShortPlan &s, int sm_count) {
     const int groups = p.n_kv / s.hw, per = s.per_sm * sm_count / groups;
     return (per < 1 ? 1 : per) * groups;
@@ -838,6 +890,7 @@ struct ShortCall {
     int dtype, grid, only_short;
     uint32_t polls;
     float *ws;
+    uint32_t *counters;
     bool tma, pdl;
     cudaStream_t stream;
 };
@@ -865,15 +918,16 @@ cudaError_t encode_maps(const AttnQuant &p, int hw, ShortMaps *m) {
 
 template <int HD, int RB, int TERMS, int HW, int NST, bool TMA>
 cudaError_t launch_short(const AttnQuant &p, const ShortCall &c) {
+    constexpr size_t joins = (size_t)SH_JOIN * HW * RB * sizeof(float2);
     constexpr size_t meet = HW == SH_WARPS ? 0 : (size_t)SH_WARPS * RB * (16 + 2) * sizeof(float);
     using St = ShortStage<HD, HW>;
-    constexpr size_t smem = NST * (St::BYTES + St::AUX) + meet;
+    constexpr size_t smem = NST * (St::BYTES + St::AUX) + joins + meet;
     static_assert(2 * (smem + 2048) <= 228 * 1024, "two CTAs' shared memory");
     auto k = attention_quant_short_kernel<HD, RB, TERMS, HW, NST, TMA>;
     const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;
     return launch_dependent(k, dim3((unsigned)c.grid), dim3(SH_THREADS + (TMA ? 32 : 128)), smem, c.stream, c.pdl, c.maps, p,
-                            (int)(c.dtype == DT_BF16), c.only_short, c.polls, c.ws);
+                            (int)(c.dtype == DT_BF16), c.only_short, c.polls, c.ws, c.counters);
 }
 template <int HD, int RB, int TERMS, int NST>
 cudaError_t launch_short_hw(const AttnQuant &p, int hw, const ShortCall &c) {
@@ -885,17 +939,12 @@ cudaError_t launch_short_hw(const AttnQuant &p, int hw, const ShortCall &c) {
 }
 template <int HD>
 cudaError_t launch_short_all(const AttnQuant &p, const ShortPlan &pl, const ShortCall &c) {
-    cudaError_t e;
     constexpr int NST = HD == 128 ? 3 : 5;
-    if (pl.terms == 2) e = pl.rb == 8 ? launch_short_hw<HD, 8, 2, NST>(p, pl.hw, c) : launch_short_hw<HD, 16, 2, NST>(p, pl.hw, c);
-    else e = pl.rb == 8 ? launch_short_hw<HD, 8, 1, NST>(p, pl.hw, c) : launch_short_hw<HD, 16, 1, NST>(p, pl.hw, c);
-    if (e != cudaSuccess) return e;
-    const Rows rows{pl.rb, 16 * SH_TILES / pl.hw, pl.hw, c.only_short};
-    return launch_dependent(attention_quant_merge_kernel<HD>, dim3((unsigned)p.total_q * p.n_heads), dim3(MERGE_THREADS), 0, c.stream, c.pdl,
-                            p, (int)(c.dtype == DT_BF16), rows, c.grid / (p.n_kv / pl.hw), (const float *)c.ws);
+    if (pl.terms == 2) return pl.rb == 8 ? launch_short_hw<HD, 8, 2, NST>(p, pl.hw, c) : launch_short_hw<HD, 16, 2, NST>(p, pl.hw, c);
+    return pl.rb == 8 ? launch_short_hw<HD, 8, 1, NST>(p, pl.hw, c) : launch_short_hw<HD, 16, 1, NST>(p, pl.hw, c);
 }
 
-bool mma_supported(const AttnQuant &p) { return p.head_dim == 64 || p.head_dim == 128; }
+bool mma_supported(const AttnQuant &p) { return (p.head_dim == 64 || p.head_dim == 128) && p.n_kv <= SHORT_MAX_GROUPS; }
 
 }  // namespace
 
@@ -903,7 +952,10 @@ size_t attention_quant_workspace(const AttnQuant &p, int dtype, int sm_count) {
     return mma_supported(p) ? short_workspace(p, short_plan(p, dtype), sm_count) : 0;
 }
 
-cudaError_t launch_attention_quant(const AttnQuant &p, int dtype, float *ws, int sm_count, uint32_t polls, cudaStream_t s,
+// Two levels x two parts a CTA; a call with more head groups than resident CTAs has a CTA each.
+size_t attention_quant_counter_bytes(int sm_count) { return (size_t)4 * (2 * sm_count > SHORT_MAX_GROUPS ? 2 * sm_count : SHORT_MAX_GROUPS) * sizeof(uint32_t); }
+
+cudaError_t launch_attention_quant(const AttnQuant &p, int dtype, float *ws, uint32_t *counters, int sm_count, uint32_t polls, cudaStream_t s,
                                    bool pdl, uint64_t *launches) {
     if (p.total_q <= 0 || p.num_req <= 0) return cudaSuccess;
     if (!mma_supported(p)) {
@@ -913,13 +965,13 @@ cudaError_t launch_attention_quant(const AttnQuant &p, int dtype, float *ws, int
     }
     const ShortPlan pl = short_plan(p, dtype);
     ShortCall c = {};
-    c.dtype = dtype; c.grid = short_grid(p, pl, sm_count); c.polls = polls; c.ws = ws; c.pdl = pdl; c.stream = s;
+    c.dtype = dtype; c.grid = short_grid(p, pl, sm_count); c.polls = polls; c.ws = ws; c.counters = counters; c.pdl = pdl; c.stream = s;
     c.tma = tma_fits(p);
     if (c.tma) {
         const cudaError_t e = encode_maps(p, pl.hw, &c.maps);
         if (e != cudaSuccess) return e;
     }
-    *launches += 2;
+    ++*launches;
     return p.head_dim == 128 ? launch_short_all<128>(p, pl, c) : launch_short_all<64>(p, pl, c);
 }
 

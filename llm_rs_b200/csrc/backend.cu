@@ -62,6 +62,7 @@ struct llmrs_ctx {
     float conv_norm_eps = 0.0f;
     float *att_ws = nullptr;         // partial results of attention over split sequences
     size_t att_ws_bytes = 0;
+    uint32_t *quant_counters = nullptr;    // of attention_quant's joining of split sequences (zero between launches)
     uint32_t *argmax_out = nullptr;  // device word argmax writes its result to
     uint32_t *tokens = nullptr;      // device copy of embed's token ids
     // GGUF uploads: two pinned host pieces, two device pieces (raw Q6_K before its re-layout), one event each
@@ -109,6 +110,7 @@ struct llmrs_ctx {
         if (code == 0) return LLMRS_OK;
         cudaMemset(dev_error, 0, 2 * sizeof code);
         if (split_ws) cudaMemset(split_ws, 0, gemm_split_counter_bytes());     // an abandoned launch may have left counters behind
+        if (quant_counters) cudaMemset(quant_counters, 0, attention_quant_counter_bytes(sm_count));
         if (code == 8) return fail(LLMRS_ERR_ARG, "%s: an index of an 8-bit cache call named a slot, page or length beyond the pool or the page table", what);
         if (code == 7) return fail(LLMRS_ERR_ARG, "%s: embed was given a token id beyond the table", what);
         return fail(LLMRS_ERR_KERNEL, "%s: a kernel gave up a bounded wait (code %u); results are incomplete", what, code);
@@ -383,6 +385,8 @@ int llmrs_cuda_create(int device, void *stream, llmrs_ctx **out) {
     if (e == cudaSuccess) e = cudaMalloc((void **)&ctx->argmax_out, sizeof(uint32_t));
     if (e == cudaSuccess) e = cudaMalloc(&ctx->split_ws, gemm_split_workspace_bytes(ctx->sm_count));
     if (e == cudaSuccess) e = cudaMemset(ctx->split_ws, 0, gemm_split_counter_bytes());
+    if (e == cudaSuccess) e = cudaMalloc((void **)&ctx->quant_counters, attention_quant_counter_bytes(ctx->sm_count));
+    if (e == cudaSuccess) e = cudaMemset(ctx->quant_counters, 0, attention_quant_counter_bytes(ctx->sm_count));
     if (e != cudaSuccess) {
         g_create_error = cudaGetErrorString(e);
         llmrs_cuda_destroy(ctx);
@@ -405,6 +409,7 @@ int llmrs_cuda_destroy(llmrs_ctx *ctx) {
     if (ctx->tokens) cudaFree(ctx->tokens);
     if (ctx->argmax_out) cudaFree(ctx->argmax_out);
     if (ctx->att_ws) cudaFree(ctx->att_ws);
+    if (ctx->quant_counters) cudaFree(ctx->quant_counters);
     if (ctx->norm_tmp) cudaFree(ctx->norm_tmp);
     for (void *old : ctx->retired) cudaFree(old);
     for (auto &op : ctx->perf_ops) { cudaEventDestroy(op.a); cudaEventDestroy(op.b); }
@@ -1333,7 +1338,7 @@ int llmrs_cuda_attention_quant(llmrs_ctx *ctx, llmrs_buf *out, const llmrs_buf *
     e = ctx->begin_work();
     PerfScope perf(ctx, name, 2.0 * buf_elems(q) * dense_elem_bytes(q->dtype), 0.0);    // q and out: the lengths live on the device
     if (e == cudaSuccess)
-        e = launch_attention_quant(p, (int)q->dtype, ctx->att_ws, ctx->sm_count, ctx->mbar_polls, ctx->stream, ctx->pdl, &ctx->launches);
+        e = launch_attention_quant(p, (int)q->dtype, ctx->att_ws, ctx->quant_counters, ctx->sm_count, ctx->mbar_polls, ctx->stream, ctx->pdl, &ctx->launches);
     if (e != cudaSuccess) return ctx->cuda_fail(e, name);
     return LLMRS_OK;
 }

@@ -143,8 +143,9 @@ struct AttnQuant {
     int total_q, num_req, n_heads, n_kv, head_dim, block_size, max_blocks;
 };
 size_t attention_quant_workspace(const AttnQuant &p, int dtype, int sm_count);      // bytes of `ws`
-cudaError_t launch_attention_quant(const AttnQuant &p, int dtype, float *ws, int sm_count, uint32_t polls, cudaStream_t s,
-                                   bool pdl, uint64_t *launches);
+size_t attention_quant_counter_bytes(int sm_count);      // of `counters`: zero before the first launch, left zero by each
+cudaError_t launch_attention_quant(const AttnQuant &p, int dtype, float *ws, uint32_t *counters, int sm_count,
+                                   uint32_t polls, cudaStream_t s, bool pdl, uint64_t *launches);
 
 // Decode matmul: integer dot products per scale group, float32 across groups; any M (tokens are
 // processed in passes of <= 4).  x_dtype / out_dtype are DT_F32 or DT_BF16.  err_word names the device

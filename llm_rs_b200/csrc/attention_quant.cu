@@ -12,6 +12,7 @@
 #include "llmrs_common.cuh"
 #include "pipeline.cuh"
 #include "tensor_map.h"
+#include "umma.cuh"
 
 namespace llmrs {
 
@@ -893,6 +894,501 @@ attention_quant_short_kernel(const __grid_constant__ ShortMaps maps, const AttnQ
     }
 }
 
+// ---- many rows: prompts and chunks of prompts -------------------------------------------------------
+// Bound by the tensor cores (tcgen05, f16 operands, float32 accumulators in TMEM), then by the exponentials: a score costs
+// 4 head_dim operations, 512 of a tensor core's cycles for 128 x 128 of them, and one ex2, 1024 cycles of the
+// SM's 16 a cycle.  So a CTA keeps two tiles of 128 query rows (token x head of the group, packed) against one
+// stream of keys and values: while one tile's weights are formed the tensor cores work for the other.
+//
+//   warps 0-3, 4-7   weights of tile 0, 1: a thread owns a row.  Scores come from TMEM 32 columns at a time, once for the
+//                    maximum and once for the weights, which go back as f16 over the scores that they came from.
+//   warps 8-11       keys and values: codes from memory to registers, one tile ahead, to f16 (exact), to shared memory in
+//                    the 128-byte swizzle; the scales, ready for use.  Any page size: rows are looked up one by one.
+//   warp 12          issues the products: S = Q K^T (both from shared memory), O += W V (W from TMEM; the values lie
+//                    as they come, positions in rows, so they are the operand's major dimension the other way round).
+//
+// Softmax in one pass: O and the sum refer to a maximum that is only moved when a row's grows by more than 2 (log2), so O
+// is rarely rescaled; weights then stay below 4, and enter as e^(s - m) vs / R * 2^13 (R as in the other kernel).
+constexpr int LG_ROWS = 128, LG_POS = 128, LG_THREADS = 13 * 32;
+constexpr float LG_SLACK = 2.0f;     // log2: the weights' factor 2^13 leaves two octaves to f16's 65504
+
+template <int HD> struct LongSmem {
+    static constexpr int HALVES = HD / 64, TILE = LG_ROWS * HD * 2;      // 128 rows of f16, in halves of 64 dimensions
+    static constexpr int Q = 0, K = 2 * TILE, V = K + 2 * TILE, SC = V + 2 * TILE;
+    // scales of a tile of positions: ks [128], vs / R * 2^13 [128], which positions are there [4], all there, R's bits
+    static constexpr int STAGES = 3, KS = 0, VW = 512, MASK = 1024, ALL = 1040, RBITS = 1044, SCALES = 1152;
+    static constexpr int BYTES = SC + STAGES * SCALES;
+};
+
+__device__ __forceinline__ void umma_f16_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+// 32 lanes x 32 consecutive columns of TMEM -> 32 registers a thread.
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+          "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
+          "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]),
+          "=r"(r[31])
+        : "r"(taddr)
+        : "memory");
+}
+// Pairs of floats in one instruction.
+__device__ __forceinline__ float2 pair_op(float2 a, float2 b, float2 c) {
+    float2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;"
+        : "=l"(reinterpret_cast<unsigned long long &>(r))
+        : "l"(reinterpret_cast<unsigned long long &>(a)), "l"(reinterpret_cast<unsigned long long &>(b)), "l"(reinterpret_cast<unsigned long long &>(c)));
+    return r;
+}
+__device__ __forceinline__ float2 pair_mul(float2 a, float2 b) {
+    float2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;"
+        : "=l"(reinterpret_cast<unsigned long long &>(r))
+        : "l"(reinterpret_cast<unsigned long long &>(a)), "l"(reinterpret_cast<unsigned long long &>(b)));
+    return r;
+}
+__device__ __forceinline__ float2 pair_add(float2 a, float2 b) {
+    float2 r;
+    asm("add.rn.f32x2 %0, %1, %2;"
+        : "=l"(reinterpret_cast<unsigned long long &>(r))
+        : "l"(reinterpret_cast<unsigned long long &>(a)), "l"(reinterpret_cast<unsigned long long &>(b)));
+    return r;
+}
+// Shared-memory descriptor of an operand whose major dimension is not the summed one (values: rows are positions, which are
+// summed over, 64 dimensions of f16 to a 128-byte row, 128-byte swizzle): 8 rows are 1024 bytes (stride offset), the
+// next 64 dimensions `half_bytes` further (leading offset).
+__device__ __forceinline__ uint64_t umma_desc_sw128_mn(uint32_t smem_addr, uint32_t half_bytes) {
+    uint64_t d = 0;
+    d |= (uint64_t)((smem_addr >> 4) & 0x3FFF);
+    d |= (uint64_t)(half_bytes >> 4) << 16;
+    d |= (uint64_t)(1024 >> 4) << 32;
+    d |= (uint64_t)1 << 46;
+    d |= (uint64_t)2 << 61;
+    return d;
+}
+// Where 16-byte chunk c (8 f16) of row `row` of a 128-row tile lies: halves of 64 dimensions, 128-byte swizzle.
+__device__ __forceinline__ int f16_chunk_at(int row, int c) { return (c >> 3) * (128 * 128) + row * 128 + 16 * ((c & 7) ^ (row & 7)); }
+
+template <int HD>
+__global__ void __launch_bounds__(LG_THREADS, 1)
+attention_quant_long_kernel(const AttnQuant p, int skip_short, uint32_t polls) {
+    using Sm = LongSmem<HD>;
+    constexpr int CH = HD / 16;                          // 16-byte chunks of codes in a row
+    extern __shared__ __align__(1024) uint8_t lg_smem[];
+    __shared__ __align__(8) uint64_t q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], sc_full[Sm::STAGES], sc_empty[Sm::STAGES], s_full[2], p_full[2], o_full[2];
+    __shared__ uint32_t tmem_base_s, vmax_s[2][4], gone_s[2][4];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    if (tid == 0) {
+        for (int i = 0; i < 2; i++) {
+            mbar_init(&q_full[i], 128);
+            mbar_init(&k_full[i], 128);
+            mbar_init(&k_empty[i], 1);
+            mbar_init(&v_full[i], 128);
+            mbar_init(&v_empty[i], 1);
+            mbar_init(&s_full[i], 1);
+            mbar_init(&p_full[i], 128);
+            mbar_init(&o_full[i], 1);
+        }
+        for (int i = 0; i < Sm::STAGES; i++) {
+            mbar_init(&sc_full[i], 128);
+            mbar_init(&sc_empty[i], 8);
+        }
+        mbar_init_fence();
+    }
+    pdl_prologue();
+    // ---- which 256 rows: blocks of the requests in order, of a request the last (longest) ones first, KV heads innermost ----
+    const int group = p.n_heads / p.n_kv, kvh = blockIdx.x % p.n_kv;
+    int want = blockIdx.x / p.n_kv, req = -1;
+    Request r = {0, 0, 0};
+    for (int q0 = 0; q0 < p.num_req && req < 0; q0 += 32) {
+        Request mine = {0, 0, 0};
+        int blocks = 0;
+        if (q0 + lane < p.num_req) {
+            mine = request_of(p, q0 + lane);
+            const long long rows = (long long)mine.count * group;
+            blocks = skip_short && rows <= SHORT_ROWS ? 0 : (int)((rows + 2 * LG_ROWS - 1) / (2 * LG_ROWS));
+        }
+        int inc = blocks;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= o) inc += v;
+        }
+        const unsigned hit = __ballot_sync(0xffffffffu, want < inc);
+        if (hit) {
+            const int src = __ffs(hit) - 1;
+            req = q0 + src;
+            r.first = __shfl_sync(0xffffffffu, mine.first, src);
+            r.count = __shfl_sync(0xffffffffu, mine.count, src);
+            r.before = __shfl_sync(0xffffffffu, mine.before, src);
+            want = __shfl_sync(0xffffffffu, inc, src) - 1 - want;
+        } else {
+            want -= __shfl_sync(0xffffffffu, inc, 31);
+        }
+    }
+    if (req < 0) return;                                 // the grid holds as many CTAs as any batch of this size can need
+    const int row0 = want * 2 * LG_ROWS, rows = r.count * group - row0;          // of this CTA: 1 .. 256 are used
+    // positions that tile t's last row sees, and tiles of positions
+    int nt[2];
+#pragma unroll
+    for (int t = 0; t < 2; t++) {
+        const int n = min(rows - t * LG_ROWS, LG_ROWS);
+        const int end = n > 0 ? r.before + (row0 + t * LG_ROWS + n - 1) / group + 1 : 0;
+        nt[t] = end > 0 ? (end + LG_POS - 1) / LG_POS : 0;
+    }
+    const int n_tiles = max(nt[0], nt[1]);               // tile 1's rows come later and see more, if there are any
+    const int kv_end = r.before + (row0 + min(rows, 2 * LG_ROWS) - 1) / group + 1;
+    if (warp == 12) { tmem_alloc(&tmem_base_s, 512); tmem_relinquish(); }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_base_s;                   // scores of tile t at 128 t, O at 256 + 128 t
+    bool dead = false;
+    auto wait = [&](uint64_t *bar, uint32_t parity, uint32_t code) {     // gives up once; then nothing is waited for any more
+        if (!dead && !mbar_wait(bar, parity, polls)) { dead = true; report_error(p.err, code); }
+    };
+
+    if (warp < 8) {
+        // ================= weights =================
+        const int t = warp >> 2, i = tid & 127, rr = row0 + t * LG_ROWS + i;
+        const bool on = t * LG_ROWS + i < rows;
+        const int len = on ? r.before + rr / group + 1 : 0;
+        const int min_len = r.before + (row0 + t * LG_ROWS) / group + 1;         // what the tile's first row sees
+        const bool full_tile = rows >= (t + 1) * LG_ROWS;
+        const size_t off = on ? ((size_t)(r.first + rr / group) * p.n_heads + (size_t)kvh * group + rr % group) * HD : 0;
+        // the row of queries: its size, then scaled by a power of two to f16 and into the operand's layout
+        float amax = 0.0f;
+        const uint16_t *q = (const uint16_t *)p.q + off;
+#pragma unroll 4
+        for (int c = 0; c < HD / 8; c++) {
+            const uint4 u = on ? *reinterpret_cast<const uint4 *>(q + 8 * c) : make_uint4(0, 0, 0, 0);
+            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+            for (int x = 0; x < 4; x++) amax = fmaxf(amax, fmaxf(fabsf(__uint_as_float(w[x] << 16)), fabsf(__uint_as_float(w[x] & 0xFFFF0000u))));
+        }
+        const int ex = row_exponent(amax);
+        const float up = exp2i(ex), c_row = exp2i(-ex) * (1.4426950408889634f / sqrtf((float)HD));
+#pragma unroll 4
+        for (int c = 0; c < HD / 8; c++) {
+            const uint4 u = on ? *reinterpret_cast<const uint4 *>(q + 8 * c) : make_uint4(0, 0, 0, 0);
+            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+            uint32_t h[4];
+#pragma unroll
+            for (int x = 0; x < 4; x++) h[x] = pack_f16(__uint_as_float(w[x] << 16) * up, __uint_as_float(w[x] & 0xFFFF0000u) * up);
+            *reinterpret_cast<uint4 *>(lg_smem + Sm::Q + t * Sm::TILE + f16_chunk_at(i, c)) = make_uint4(h[0], h[1], h[2], h[3]);
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        mbar_arrive(&q_full[t]);
+
+        const uint32_t lane_base = tmem + ((uint32_t)(warp & 3) << 21);          // this warp's 32 lanes
+        const uint32_t s_col = lane_base + 128 * t, o_col = lane_base + 256 + 128 * t;
+        float m_ref = -INFINITY;
+        float2 l2 = make_float2(0.0f, 0.0f);
+        uint32_t r_bits = 17u << 23;
+        for (int j = 0; j < n_tiles; j++) {
+            const int st = j % Sm::STAGES;
+            wait(&sc_full[st], (j / Sm::STAGES) & 1, KERR_FULL_WAIT);
+            if (j < nt[t]) {
+                const uint8_t *sc = lg_smem + Sm::SC + st * Sm::SCALES;
+                const float *ks = reinterpret_cast<const float *>(sc + Sm::KS), *vw = reinterpret_cast<const float *>(sc + Sm::VW);
+                const uint32_t r_new = *reinterpret_cast<const uint32_t *>(sc + Sm::RBITS);
+                const bool masked = !full_tile || (j + 1) * LG_POS > min_len || *reinterpret_cast<const uint32_t *>(sc + Sm::ALL) == 0;
+                wait(&s_full[t], j & 1, KERR_MMA_WAIT);
+                tc_fence_after();
+                auto bits_of = [&](int c) -> uint32_t {  // which of the 32 positions of chunk c this row sees
+                    const int n = len - j * LG_POS - 32 * c;
+                    const uint32_t there = *reinterpret_cast<const uint32_t *>(sc + Sm::MASK + 4 * c);
+                    return n <= 0 ? 0u : n >= 32 ? there : there & ((1u << n) - 1);
+                };
+                // ---- the row's maximum ----
+                float mx0 = -INFINITY, mx1 = -INFINITY;
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    uint32_t v[32];
+                    tmem_ld32(s_col + 32 * c, v);
+                    tmem_ld_wait();
+                    if (!masked) {
+#pragma unroll
+                        for (int x = 0; x < 32; x += 4) {
+                            const float4 k4 = *reinterpret_cast<const float4 *>(ks + 32 * c + x);
+                            const float2 a = pair_mul(make_float2(__uint_as_float(v[x]), __uint_as_float(v[x + 1])), make_float2(k4.x, k4.y));
+                            const float2 b = pair_mul(make_float2(__uint_as_float(v[x + 2]), __uint_as_float(v[x + 3])), make_float2(k4.z, k4.w));
+                            mx0 = fmaxf(mx0, fmaxf(a.x, a.y));
+                            mx1 = fmaxf(mx1, fmaxf(b.x, b.y));
+                        }
+                    } else {
+                        const uint32_t bits = bits_of(c);
+#pragma unroll
+                        for (int x = 0; x < 32; x++) {
+                            const float a = __uint_as_float(v[x]) * ks[32 * c + x];
+                            mx0 = fmaxf(mx0, bits >> x & 1 ? a : -INFINITY);
+                        }
+                    }
+                }
+                const float mx = fmaxf(mx0, mx1) * c_row;
+                // ---- move the reference, O and the sum where the maximum has outgrown it ----
+                const float m_new = mx > m_ref + LG_SLACK ? mx : m_ref;          // m_ref = -inf: any score at all
+                const bool moved = m_new != m_ref || r_new != r_bits;
+                const float base = m_new == -INFINITY ? 0.0f : m_new;
+                if (j > 0 && __any_sync(0xffffffffu, moved)) {
+                    const float f = m_new == m_ref ? 1.0f : ex2(m_ref - base);
+                    const float sh = r_new - r_bits >= (127u << 23) ? 0.0f : __uint_as_float(r_bits - r_new + (127u << 23));  // R / R'
+                    l2.x *= f;
+                    l2.y *= f;
+#pragma unroll
+                    for (int c = 0; c < HD / 32; c++) {
+                        uint32_t v[32];
+                        tmem_ld32(o_col + 32 * c, v);
+                        tmem_ld_wait();
+                        uint32_t a[16], b[16];
+#pragma unroll
+                        for (int x = 0; x < 16; x++) {
+                            a[x] = __float_as_uint(__uint_as_float(v[x]) * (f * sh));
+                            b[x] = __float_as_uint(__uint_as_float(v[16 + x]) * (f * sh));
+                        }
+                        tmem_st16(o_col + 32 * c, a);
+                        tmem_st16(o_col + 32 * c + 16, b);
+                    }
+                }
+                m_ref = m_new;
+                r_bits = r_new;
+                // ---- the weights, over the scores ----
+                const float2 c2 = make_float2(c_row, c_row), nb = make_float2(-base, -base);
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    uint32_t v[32], w[16];
+                    tmem_ld32(s_col + 32 * c, v);
+                    tmem_ld_wait();
+                    const uint32_t bits = masked ? bits_of(c) : 0xFFFFFFFFu;
+#pragma unroll
+                    for (int x = 0; x < 32; x += 4) {
+                        const float4 k4 = *reinterpret_cast<const float4 *>(ks + 32 * c + x), w4 = *reinterpret_cast<const float4 *>(vw + 32 * c + x);
+#pragma unroll
+                        for (int y = 0; y < 2; y++) {
+                            const float2 k2 = y ? make_float2(k4.z, k4.w) : make_float2(k4.x, k4.y);
+                            const float2 w2 = y ? make_float2(w4.z, w4.w) : make_float2(w4.x, w4.y);
+                            const int at = x + 2 * y;
+                            float2 e = pair_op(pair_mul(make_float2(__uint_as_float(v[at]), __uint_as_float(v[at + 1])), k2), c2, nb);
+                            e.x = ex2(e.x);
+                            e.y = ex2(e.y);
+                            if (masked) {
+                                if (!(bits >> at & 1)) e.x = 0.0f;
+                                if (!(bits >> (at + 1) & 1)) e.y = 0.0f;
+                            }
+                            l2 = pair_add(l2, e);
+                            e = pair_mul(e, w2);
+                            if (masked) {                // not 0 * NaN
+                                if (!(bits >> at & 1)) e.x = 0.0f;
+                                if (!(bits >> (at + 1) & 1)) e.y = 0.0f;
+                            }
+                            w[at / 2] = pack_f16(e.x, e.y);
+                        }
+                    }
+                    tmem_st16(s_col + 16 * c, w);
+                }
+                tmem_st_wait();
+                tc_fence_before();
+                mbar_arrive(&p_full[t]);
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sc_empty[st]);
+        }
+        // ---- O, divided by the sum ----
+        const float l = l2.x + l2.y;
+        const float norm = l == 0.0f ? 0.0f : __uint_as_float(r_bits - (13u << 23)) / l;
+        uint16_t *out = (uint16_t *)p.out + off;
+        if (nt[t] > 0) {
+            wait(&o_full[t], 0, KERR_MMA_WAIT);
+            tc_fence_after();
+        }
+#pragma unroll
+        for (int c = 0; c < HD / 32; c++) {
+            uint32_t v[32];
+            if (nt[t] > 0) {
+                tmem_ld32(o_col + 32 * c, v);
+                tmem_ld_wait();
+            }
+            if (!on) continue;
+#pragma unroll
+            for (int x = 0; x < 32; x += 8) {
+                uint32_t h[4];
+#pragma unroll
+                for (int y = 0; y < 4; y++) {
+                    // rows without positions: zeros (their columns of O may never have been written)
+                    const float a = len > 0 ? __uint_as_float(v[x + 2 * y]) * norm : 0.0f, b = len > 0 ? __uint_as_float(v[x + 2 * y + 1]) * norm : 0.0f;
+                    const __nv_bfloat162 z = __floats2bfloat162_rn(a, b);
+                    h[y] = *reinterpret_cast<const uint32_t *>(&z);
+                }
+                *reinterpret_cast<uint4 *>(out + 32 * c + x) = make_uint4(h[0], h[1], h[2], h[3]);
+            }
+        }
+        tc_fence_before();
+    } else if (warp < 12) {
+        // ================= keys and values =================
+        const int w = warp - 8;                          // this warp's positions are 32 w .. 32 w + 31 of a tile
+        const size_t kv_dim = (size_t)p.n_kv * HD;
+        const uint32_t *table = p.block_table + (size_t)req * p.max_blocks;
+        const uint8_t *kp = p.k_pool + (size_t)kvh * HD, *vp = p.v_pool + (size_t)kvh * HD;
+        const float *ksp = p.k_scales + (size_t)kvh * p.num_slots, *vsp = p.v_scales + (size_t)kvh * p.num_slots;
+        constexpr int RPI = 32 / CH, N = 32 / RPI;       // rows a pass, passes
+        const int c = lane % CH;
+        uint4 kr[N], vr[N];
+        float ks = 0.0f, vs = 0.0f;
+        uint32_t there = 0, page = 0;
+        auto page_of = [&](int j) -> uint32_t {
+            const int pos = j * LG_POS + 32 * w + lane;
+            return pos < kv_end ? table[pos / p.block_size] : 0u;
+        };
+        auto load = [&](int j) {                         // the codes and scales of tile j, and the page of the tile after it
+            const int pos = j * LG_POS + 32 * w + lane;
+            const unsigned long long s64 = (unsigned long long)page * p.block_size + (unsigned)(pos % p.block_size);
+            const bool ok = pos < kv_end && s64 < p.num_slots;
+            if (pos < kv_end && !ok) report_error(p.err, KERR_SLOT_RANGE);
+            const uint32_t slot = ok ? (uint32_t)s64 : 0u;
+            there = __ballot_sync(0xffffffffu, ok);
+            ks = ok ? __ldg(ksp + slot) : 0.0f;
+            vs = ok ? __ldg(vsp + slot) : 0.0f;
+#pragma unroll
+            for (int x = 0; x < N; x++) {
+                const int row = x * RPI + lane / CH;
+                const size_t at = (size_t)__shfl_sync(0xffffffffu, slot, row) * kv_dim + 16 * c;
+                const bool on = there >> row & 1;
+                kr[x] = on ? ldg128(kp + at) : make_uint4(0, 0, 0, 0);
+                vr[x] = on ? ldg128(vp + at) : make_uint4(0, 0, 0, 0);
+            }
+            page = page_of(j + 1);
+        };
+        auto store = [&](uint8_t *tile, const uint4 (&raw)[N]) {
+#pragma unroll
+            for (int x = 0; x < N; x++) {
+                const int row = 32 * w + x * RPI + lane / CH;
+                uint32_t h[8];
+                codes_to_f16(raw[x].x, h[0], h[1]);
+                codes_to_f16(raw[x].y, h[2], h[3]);
+                codes_to_f16(raw[x].z, h[4], h[5]);
+                codes_to_f16(raw[x].w, h[6], h[7]);
+                *reinterpret_cast<uint4 *>(tile + f16_chunk_at(row, 2 * c)) = make_uint4(h[0], h[1], h[2], h[3]);
+                *reinterpret_cast<uint4 *>(tile + f16_chunk_at(row, 2 * c + 1)) = make_uint4(h[4], h[5], h[6], h[7]);
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        };
+        uint32_t r_bits = 17u << 23;
+        if (n_tiles > 0) {
+            page = page_of(0);
+            load(0);
+        }
+        for (int j = 0; j < n_tiles; j++) {
+            const int b = j & 1, st = j % Sm::STAGES;
+            const uint32_t par = ((j >> 1) & 1) ^ 1;
+            // scales, with R the least power of two that no vs so far exceeds
+            float vmax = fmaxf(0.0f, vs);
+#pragma unroll
+            for (int o = 16; o; o >>= 1) vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, o));
+            if (lane == 0) {
+                vmax_s[b][w] = __float_as_uint(vmax);
+                gone_s[b][w] = there != 0xFFFFFFFFu;     // positions past kv_end, or on a page beyond the pool
+            }
+            if (j >= 2) wait(&k_empty[b], par, KERR_EMPTY_WAIT);
+            store(lg_smem + Sm::K + b * Sm::TILE, kr);
+            mbar_arrive(&k_full[b]);
+            if (j >= Sm::STAGES) wait(&sc_empty[st], ((j / Sm::STAGES) & 1) ^ 1, KERR_EMPTY_WAIT);
+            named_barrier_sync(2, 128);                  // what the four warps have found
+            const uint32_t top = max(max(vmax_s[b][0], vmax_s[b][1]), max(vmax_s[b][2], vmax_s[b][3]));
+            r_bits = max(r_bits, min((top + 0x7FFFFFu) & 0x7F800000u, 253u << 23));
+            uint8_t *sc = lg_smem + Sm::SC + st * Sm::SCALES;
+            reinterpret_cast<float *>(sc + Sm::KS)[32 * w + lane] = ks;
+            reinterpret_cast<float *>(sc + Sm::VW)[32 * w + lane] = vs * __uint_as_float(((127u + 127u + 13u) << 23) - r_bits);       // 2^13 / R
+            if (lane == 0) reinterpret_cast<uint32_t *>(sc + Sm::MASK)[w] = there;
+            if (tid == 8 * 32) {
+                *reinterpret_cast<uint32_t *>(sc + Sm::ALL) = !(gone_s[b][0] | gone_s[b][1] | gone_s[b][2] | gone_s[b][3]);
+                *reinterpret_cast<uint32_t *>(sc + Sm::RBITS) = r_bits;
+            }
+            mbar_arrive(&sc_full[st]);
+            if (j >= 2) wait(&v_empty[b], par, KERR_EMPTY_WAIT);
+            store(lg_smem + Sm::V + b * Sm::TILE, vr);
+            mbar_arrive(&v_full[b]);
+            if (j + 1 < n_tiles) load(j + 1);
+        }
+    } else {
+        // ================= products =================
+        constexpr uint32_t QK_DESC = umma_idesc_f16(LG_POS);             // N = 128 positions, K-major both
+        constexpr uint32_t PV_DESC = umma_idesc_f16(HD) | (1u << 16);    // N = head_dim; the values' major dimension is N
+        const uint32_t base = smem_u32(lg_smem);
+        const bool one = elect_one();
+        auto scores = [&](int t, int j) {
+            if (one && !dead) {
+#pragma unroll
+                for (int k = 0; k < HD / 16; k++) {
+                    const uint32_t step = (k >> 2) * (128 * 128) + (k & 3) * 32;
+                    umma_f16_ss(tmem + 128 * t, umma_desc_sw128(base + Sm::Q + t * Sm::TILE + step),
+                                umma_desc_sw128(base + Sm::K + (j & 1) * Sm::TILE + step), QK_DESC, k > 0);
+                }
+                umma_commit(&s_full[t]);
+            }
+            __syncwarp();
+        };
+        for (int t = 0; t < 2; t++) wait(&q_full[t], 0, KERR_FULL_WAIT);
+        if (n_tiles > 0) {
+            wait(&k_full[0], 0, KERR_FULL_WAIT);
+            tc_fence_after();
+            for (int t = 0; t < 2; t++)
+                if (nt[t] > 0) scores(t, 0);
+            if (one && !dead) umma_commit(&k_empty[0]);
+            __syncwarp();
+        }
+        for (int j = 0; j < n_tiles; j++) {
+            wait(&v_full[j & 1], (j >> 1) & 1, KERR_FULL_WAIT);
+            if (j + 1 < n_tiles) wait(&k_full[(j + 1) & 1], ((j + 1) >> 1) & 1, KERR_FULL_WAIT);
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+                if (j >= nt[t]) continue;
+                wait(&p_full[t], j & 1, KERR_MMA_WAIT);
+                tc_fence_after();
+                if (one && !dead) {
+#pragma unroll
+                    for (int k = 0; k < LG_POS / 16; k++)
+                        umma_f16_ts(tmem + 256 + 128 * t, tmem + 128 * t + 8 * k,
+                                    umma_desc_sw128_mn(base + Sm::V + (j & 1) * Sm::TILE + k * 2048, 128 * 128), PV_DESC, j > 0 || k > 0);
+                    if (j + 1 == nt[t]) umma_commit(&o_full[t]);
+                }
+                __syncwarp();
+                if (j + 1 < nt[t]) scores(t, j + 1);
+            }
+            if (one && !dead) {
+                umma_commit(&v_empty[j & 1]);
+                if (j + 1 < n_tiles) umma_commit(&k_empty[(j + 1) & 1]);
+            }
+            __syncwarp();
+        }
+        // nothing of this warp's may be under way when the memory goes: the last commits have arrived
+        if (n_tiles > 0) mbar_wait(&v_empty[(n_tiles - 1) & 1], ((n_tiles - 1) >> 1) & 1, polls);
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 12) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
+template <int HD>
+cudaError_t launch_long(const AttnQuant &p, int skip_short, uint32_t polls, cudaStream_t s, bool pdl) {
+    const int group = p.n_heads / p.n_kv;
+    const long long blocks = ((long long)p.total_q * group + 2 * LG_ROWS - 1) / (2 * LG_ROWS) + p.num_req;
+    const cudaError_t e = cudaFuncSetAttribute(attention_quant_long_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, LongSmem<HD>::BYTES);
+    if (e != cudaSuccess) return e;
+    if (blocks * p.n_kv > 0x7FFFFFFFll) return cudaErrorInvalidValue;
+    return launch_dependent(attention_quant_long_kernel<HD>, dim3((unsigned)(blocks * p.n_kv)), dim3(LG_THREADS), LongSmem<HD>::BYTES, s, pdl, p,
+                            skip_short, polls);
+}
+
 struct ShortPlan { int rb, terms, hw, per_sm; };
 ShortPlan short_plan(const AttnQuant &p, int dtype) {
     const int group = p.n_heads / p.n_kv;
@@ -997,6 +1493,18 @@ cudaError_t launch_attention_quant(const AttnQuant &p, int dtype, float *ws, uin
     if (c.tma) {
         const cudaError_t e = encode_maps(p, pl.hw, &c.maps);
         if (e != cudaSuccess) return e;
+    }
+    // Requests of more than 16 rows go to the long kernel, the others to the short one, which cuts what it gets into
+    // blocks of 16 rows.  The lengths are on the device; the host knows the totals.  As many tokens as requests: a
+    // decode batch, all to the short kernel.  One request: one kernel.  F32 has no long kernel.
+    const long long rows = (long long)p.total_q * (p.n_heads / p.n_kv);
+    const bool decode = p.total_q <= p.num_req || rows <= SHORT_ROWS;
+    if (dtype == DT_BF16 && !decode) {
+        const int both = p.num_req > 1;
+        cudaError_t e = p.head_dim == 128 ? launch_long<128>(p, both, polls, s, pdl) : launch_long<64>(p, both, polls, s, pdl);
+        ++*launches;
+        if (e != cudaSuccess || !both) return e;
+        c.only_short = 1;
     }
     ++*launches;
     return p.head_dim == 128 ? launch_short_all<128>(p, pl, c) : launch_short_all<64>(p, pl, c);

@@ -306,9 +306,9 @@ def expected(q, kc, ks, vc, vs, slots, lens, news, nh, nkv, hd):
             # A weight is off by its own rounding to f16 (2^-11) and by twice the error of a score: up to 256 additions
             # each off by 2^-23 (a tensor core may cut instead of rounding) of at most sum |q k|, 2^-15 of it; the
             # exponential and the sums of weights and of weighted values over up to 2^7 partial ones, 2^-16.  Below the normal
-            # range of f16 a rounding is off by 2^-25 instead, with the largest weight at 2^15: 2^-40 a position of at most |v|
-            # (weights are at most 1 and their sum at least 1).  And float32 and bf16 end at 2^-126.
-            flush = l * 2.0 ** -40 * v.abs().amax() + 2.0 ** -126
+            # range of f16 a rounding is off by 2^-25 instead, with the largest weight at 2^13 or more: 2^-38 a position of at
+            # most |v| (the sum of the weights is at least the largest).  And float32 and bf16 end at 2^-126.
+            flush = l * 2.0 ** -38 * v.abs().amax() + 2.0 ** -126
             slack[t0:t0 + n] = (a * (2.0 ** -11 + 2.0 * 2.0 ** -15 * size + 2.0 ** -16)).reshape(n, -1) + flush
         t0 += n
     return out, slack

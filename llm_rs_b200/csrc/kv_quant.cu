@@ -23,11 +23,11 @@ namespace {
 
 constexpr int RW_THREADS = 128;
 
-// V consecutive elements between memory and float registers, in one access (V * sizeof(T) = 16, or one element).
+// V consecutive elements between memory (Raw: one access) and float registers.
 template <typename T, int V> struct Chunk;
 template <> struct Chunk<__nv_bfloat16, 8> {
-    static __device__ __forceinline__ void load(float *x, const __nv_bfloat16 *p) {
-        const uint4 u = *reinterpret_cast<const uint4 *>(p);
+    using Raw = uint4;
+    static __device__ __forceinline__ void unpack(float *x, const Raw &u) {
         const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
         for (int i = 0; i < 4; i++) {
@@ -46,20 +46,20 @@ template <> struct Chunk<__nv_bfloat16, 8> {
     }
 };
 template <> struct Chunk<float, 4> {
-    static __device__ __forceinline__ void load(float *x, const float *p) {
-        const float4 u = *reinterpret_cast<const float4 *>(p);
-        x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w;
-    }
+    using Raw = float4;
+    static __device__ __forceinline__ void unpack(float *x, const Raw &u) { x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w; }
     static __device__ __forceinline__ void store(float *p, const float *x) {
         *reinterpret_cast<float4 *>(p) = make_float4(x[0], x[1], x[2], x[3]);
     }
 };
 template <> struct Chunk<__nv_bfloat16, 1> {
-    static __device__ __forceinline__ void load(float *x, const __nv_bfloat16 *p) { x[0] = __bfloat162float(*p); }
+    using Raw = __nv_bfloat16;
+    static __device__ __forceinline__ void unpack(float *x, const Raw &u) { x[0] = __bfloat162float(u); }
     static __device__ __forceinline__ void store(__nv_bfloat16 *p, const float *x) { *p = __float2bfloat16_rn(x[0]); }
 };
 template <> struct Chunk<float, 1> {
-    static __device__ __forceinline__ void load(float *x, const float *p) { x[0] = *p; }
+    using Raw = float;
+    static __device__ __forceinline__ void unpack(float *x, const Raw &u) { x[0] = u; }
     static __device__ __forceinline__ void store(float *p, const float *x) { *p = x[0]; }
 };
 
@@ -93,136 +93,186 @@ __device__ __forceinline__ void rotate(float &a, float &b, float2 t) {
 // always in one thread, rotation in place is safe, and pair j of a unit has frequency V u + j in both.
 // The cosines and sines of a token are formed once per CTA (one per thread, angle reduced in float64: at
 // position 131072 a float32 angle has lost 7 of its fraction's bits) and shared by its 40 or so heads.
-// HBM-bound: what is read and written is what the operation cannot do without.
-template <typename T, int V, int ITER>
+// HBM-bound: what is read and written is what the operation cannot do without.  So a thread asks for the units of
+// PRE rows before anything else; the angles are formed while they are under way.
+template <typename T, int V, int ITER, int PRE>
 __global__ void __launch_bounds__(RW_THREADS) rope_write_kernel(const RopeWrite p) {
+    using C = Chunk<T, V>;
     pdl_prologue();
-    __shared__ float2 cs[256];
+    __shared__ float2 cs[128];
     const int token = blockIdx.x;
     const int half = p.rotary / 2;
-    if (p.nq + p.nk > 0) {
-        const double pos = (double)p.positions[token];
-        for (int i = threadIdx.x; i < half; i += RW_THREADS) {
-            const double turns = pos * (double)p.inv_freq[i] * 0.15915494309189533577;      // 1 / (2 pi)
-            float s, c;
-            sincospif((float)(2.0 * (turns - rint(turns))), &s, &c);
-            cs[i] = make_float2(c * p.magnitude, s * p.magnitude);
-        }
-        __syncthreads();
-    }
-    const int lpr = p.lanes_per_row, rpc = RW_THREADS / lpr;
+    const int lpr = p.lanes_per_row, rpc = RW_THREADS / lpr, stride = gridDim.y * rpc;
     const int r = threadIdx.x / lpr, l = threadIdx.x % lpr;
     const int rows = p.nq + p.nk + p.nv, units = p.head_dim / (2 * V), rot_units = half / V;
+    bool angles = p.nq + p.nk > 0, to_cache = false;
     uint32_t slot = 0;
-    bool to_cache = false;
-    if (p.slots) {
-        slot = p.slots[token];
-        to_cache = slot < p.num_slots;
-        if (!to_cache && slot != 0xFFFFFFFFu && threadIdx.x == 0) report_error(p.err, KERR_SLOT_RANGE);
-    }
-    for (int base = blockIdx.y * rpc; base < rows; base += gridDim.y * rpc) {       // the same trips for a whole warp
-        const int row = base + r;
-        const int which = row < p.nq ? 0 : row < p.nq + p.nk ? 1 : 2;
-        const int head = which == 0 ? row : which == 1 ? row - p.nq : row - p.nq - p.nk;
-        const int heads = which == 0 ? p.nq : which == 1 ? p.nk : p.nv;
-        const size_t off = ((size_t)token * heads + head) * p.head_dim;
-        const T *src = (const T *)(which == 0 ? p.q : which == 1 ? p.k : p.v);
-        const bool quant = which == 2 || (which == 1 && p.k_pool);
-        float x[ITER][2 * V];
-        int at[ITER], bt[ITER];
-        float amax = 0.0f;
-        bool finite = true;
+    for (int base = blockIdx.y * rpc; base < rows; base += stride * PRE) {       // the same trips for a whole CTA
+        typename C::Raw raw[PRE][ITER][2];
 #pragma unroll
-        for (int it = 0; it < ITER; it++) {
-            const int u = l + it * lpr;
-            const bool on = row < rows && u < units;
+        for (int k = 0; k < PRE; k++) {
+            const int row = base + k * stride + r;
+            const int which = row < p.nq ? 0 : row < p.nq + p.nk ? 1 : 2;
+            const int head = row - (which == 0 ? 0 : which == 1 ? p.nq : p.nq + p.nk), heads = which == 0 ? p.nq : which == 1 ? p.nk : p.nv;
+            const T *src = (const T *)(which == 0 ? p.q : which == 1 ? p.k : p.v) + ((size_t)token * heads + head) * p.head_dim;
 #pragma unroll
-            for (int j = 0; j < 2 * V; j++) x[it][j] = 0.0f;
-            const bool halves = p.split_half && u < rot_units && which != 2;
-            at[it] = !on ? -1 : halves ? u * V : u * 2 * V;
-            bt[it] = halves ? at[it] + half : at[it] + V;
-            if (!on) continue;
-            Chunk<T, V>::load(x[it], src + off + at[it]);
-            Chunk<T, V>::load(x[it] + V, src + off + bt[it]);
-            if (which != 2) {
-                if (halves) {
-#pragma unroll
-                    for (int j = 0; j < V; j++) rotate(x[it][j], x[it][V + j], cs[u * V + j]);
-                } else if (!p.split_half) {
-#pragma unroll
-                    for (int j = 0; j < V; j++)
-                        if (u * V + j < half) rotate(x[it][2 * j], x[it][2 * j + 1], cs[u * V + j]);
-                }
-            }
-            if (quant) {
-#pragma unroll
-                for (int j = 0; j < 2 * V; j++) {
-                    amax = fmaxf(amax, fabsf(x[it][j]));
-                    finite = finite && fabsf(x[it][j]) <= 3.402823466e38f;
-                }
-            } else {
-                T *out = (T *)(which == 0 ? p.q_out : p.k_out);
-                Chunk<T, V>::store(out + off + at[it], x[it]);
-                Chunk<T, V>::store(out + off + bt[it], x[it] + V);
+            for (int it = 0; it < ITER; it++) {
+                const int u = l + it * lpr;
+                if (row >= rows || u >= units) continue;
+                const bool halves = p.split_half && u < rot_units && which != 2;
+                const int a = halves ? u * V : u * 2 * V, b = halves ? a + half : a + V;
+                raw[k][it][0] = *reinterpret_cast<const typename C::Raw *>(src + a);
+                raw[k][it][1] = *reinterpret_cast<const typename C::Raw *>(src + b);
             }
         }
-        if (!p.slots) continue;
-        for (int o = lpr >> 1; o; o >>= 1) {
-            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-            finite = __shfl_xor_sync(0xffffffffu, (int)finite, o) && finite;
+        if (base == (int)blockIdx.y * rpc && p.slots) {
+            slot = p.slots[token];
+            to_cache = slot < p.num_slots;
+            if (!to_cache && slot != 0xFFFFFFFFu && threadIdx.x == 0) report_error(p.err, KERR_SLOT_RANGE);
         }
-        if (!quant || row >= rows || !to_cache) continue;
-        const float scale = fmaxf(amax / 448.0f, 1.17549435e-38f);
-        uint8_t *pool = (which == 1 ? p.k_pool : p.v_pool) + ((size_t)slot * heads + head) * p.head_dim;
-        float *scales = which == 1 ? p.k_scales : p.v_scales;
-        if (l == 0) scales[(size_t)head * p.num_slots + slot] = finite ? scale : __int_as_float(0x7FC00000);
+        if (angles) {
+            const double pos = (double)p.positions[token];
+            for (int i = threadIdx.x; i < half; i += RW_THREADS) {
+                const double turns = pos * (double)p.inv_freq[i] * 0.15915494309189533577;  // 1 / (2 pi)
+                float s, c;
+                sincospif((float)(2.0 * (turns - rint(turns))), &s, &c);
+                cs[i] = make_float2(c * p.magnitude, s * p.magnitude);
+            }
+            __syncthreads();
+            angles = false;
+        }
 #pragma unroll
-        for (int it = 0; it < ITER; it++) {
-            if (at[it] < 0) continue;
+        for (int k = 0; k < PRE; k++) {
+            const int row = base + k * stride + r;
+            if (base + k * stride >= rows) break;        // the whole CTA
+            const int which = row < p.nq ? 0 : row < p.nq + p.nk ? 1 : 2;
+            const int head = row - (which == 0 ? 0 : which == 1 ? p.nq : p.nq + p.nk), heads = which == 0 ? p.nq : which == 1 ? p.nk : p.nv;
+            const bool quant = which == 2 || (which == 1 && p.k_pool);
+            float x[ITER][2 * V];
+            int at[ITER], bt[ITER];
+            float amax = 0.0f;
+            bool finite = true;
 #pragma unroll
-            for (int j = 0; j < 2 * V; j++) x[it][j] = finite ? x[it][j] / scale : 0.0f;
-            store_codes<V>(pool + at[it], x[it]);
-            store_codes<V>(pool + bt[it], x[it] + V);
+            for (int it = 0; it < ITER; it++) {
+                const int u = l + it * lpr;
+                const bool on = row < rows && u < units;
+                const bool halves = p.split_half && u < rot_units && which != 2;
+                at[it] = !on ? -1 : halves ? u * V : u * 2 * V;
+                bt[it] = halves ? at[it] + half : at[it] + V;
+                if (!on) continue;
+                C::unpack(x[it], raw[k][it][0]);
+                C::unpack(x[it] + V, raw[k][it][1]);
+                if (which != 2) {
+                    if (halves) {
+#pragma unroll
+                        for (int j = 0; j < V; j++) rotate(x[it][j], x[it][V + j], cs[u * V + j]);
+                    } else if (!p.split_half) {
+#pragma unroll
+                        for (int j = 0; j < V; j++)
+                            if (u * V + j < half) rotate(x[it][2 * j], x[it][2 * j + 1], cs[u * V + j]);
+                    }
+                }
+                if (quant) {
+#pragma unroll
+                    for (int j = 0; j < 2 * V; j++) {
+                        amax = fmaxf(amax, fabsf(x[it][j]));
+                        finite = finite && fabsf(x[it][j]) <= 3.402823466e38f;
+                    }
+                } else {
+                    T *out = (T *)(which == 0 ? p.q_out : p.k_out) + ((size_t)token * heads + head) * p.head_dim;
+                    C::store(out + at[it], x[it]);
+                    C::store(out + bt[it], x[it] + V);
+                }
+            }
+            if (!p.slots || !__any_sync(0xffffffffu, quant && row < rows)) continue;
+            for (int o = lpr >> 1; o; o >>= 1) {
+                amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+                finite = __shfl_xor_sync(0xffffffffu, (int)finite, o) && finite;
+            }
+            if (!quant || row >= rows || !to_cache) continue;
+            const float scale = fmaxf(amax / 448.0f, 1.17549435e-38f);
+            uint8_t *pool = (which == 1 ? p.k_pool : p.v_pool) + ((size_t)slot * heads + head) * p.head_dim;
+            float *scales = which == 1 ? p.k_scales : p.v_scales;
+            if (l == 0) scales[(size_t)head * p.num_slots + slot] = finite ? scale : __int_as_float(0x7FC00000);
+#pragma unroll
+            for (int it = 0; it < ITER; it++) {
+                if (at[it] < 0) continue;
+#pragma unroll
+                for (int j = 0; j < 2 * V; j++) x[it][j] = finite ? x[it][j] / scale : 0.0f;
+                store_codes<V>(pool + at[it], x[it]);
+                store_codes<V>(pool + bt[it], x[it] + V);
+            }
         }
     }
 }
 
-// Rows read back: out[c] = codes of slot indices[c], each head's times its scale.  A thread takes V codes of
-// one head; one product and one rounding to the output type.
-template <typename T, int V>
+// Rows read back: out[c] = codes of slot indices[c], each head's times its scale; one product and one rounding.  A thread
+// takes V codes of one head at a time (32 bytes of output, one store), of N units at once.  HBM-bound.
+template <typename T, int V> __device__ __forceinline__ void store_row(T *p, const float *x) {
+    if constexpr (V == 1) {
+        Chunk<T, 1>::store(p, x);
+    } else {
+        uint32_t w[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            if constexpr (V == 8) {
+                w[i] = __float_as_uint(x[i]);
+            } else {
+                const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+                w[i] = *reinterpret_cast<const uint32_t *>(&h);
+            }
+        }
+        asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]),
+                     "r"(w[6]), "r"(w[7])
+                     : "memory");
+    }
+}
+template <typename T, int V, int N>
 __global__ void __launch_bounds__(256)
 gather_quant_kernel(T *__restrict__ out, const uint8_t *__restrict__ pool, const float *__restrict__ scales,
                     const uint32_t *__restrict__ indices, uint32_t kv_dim, uint32_t head_dim, uint32_t num_slots,
                     uint32_t rows, uint32_t *err) {
     pdl_prologue();
     const uint32_t units = kv_dim / V;
-    const size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x;
-    if (i >= (size_t)units * rows) return;
-    const uint32_t row = (uint32_t)(i / units), d = (uint32_t)(i - (size_t)row * units) * V;
-    const uint32_t slot = indices[row];
-    if (slot >= num_slots) {                             // the row of out keeps what it held
-        if (d == 0) report_error(err, KERR_SLOT_RANGE);
-        return;
-    }
-    const uint8_t *src = pool + (size_t)slot * kv_dim + d;
-    T *dst = out + (size_t)row * kv_dim + d;
-    const float scale = scales[(size_t)(d / head_dim) * num_slots + slot];
-    float x[V];
-    if constexpr (V == 1) {
-        x[0] = __half2float(__half(__nv_cvt_fp8_to_halfraw(*src, __NV_E4M3))) * scale;
-        Chunk<T, 1>::store(dst, x);
-    } else {
-        uint32_t w[V / 4];
-        if constexpr (V == 8) { const uint2 u = *reinterpret_cast<const uint2 *>(src); w[0] = u.x; w[1] = u.y; }
-        else w[0] = *reinterpret_cast<const uint32_t *>(src);
+    const size_t first = (size_t)blockIdx.x * (256 * N) + threadIdx.x, all = (size_t)units * rows;
+    uint32_t d[N], row[N], slot[N];
 #pragma unroll
-        for (int j = 0; j < V / 2; j++) {
-            const __half2 h(__nv_cvt_fp8x2_to_halfraw2((uint16_t)(w[j / 2] >> (16 * (j & 1))), __NV_E4M3));
-            const float2 f = __half22float2(h);
-            x[2 * j] = f.x * scale;
-            x[2 * j + 1] = f.y * scale;
+    for (int k = 0; k < N; k++) {
+        const size_t i = first + k * 256;
+        row[k] = i < all ? (uint32_t)(i / units) : 0xFFFFFFFFu;
+        d[k] = (uint32_t)(i - (size_t)row[k] * units) * V;
+        slot[k] = i < all ? indices[row[k]] : 0xFFFFFFFFu;
+    }
+    uint32_t w[N][V < 4 ? 1 : V / 4];
+    float scale[N];
+#pragma unroll
+    for (int k = 0; k < N; k++) {
+        if (slot[k] >= num_slots) continue;
+        const uint8_t *src = pool + (size_t)slot[k] * kv_dim + d[k];
+        scale[k] = scales[(size_t)(d[k] / head_dim) * num_slots + slot[k]];
+        if constexpr (V == 16) { const uint4 u = *reinterpret_cast<const uint4 *>(src); w[k][0] = u.x; w[k][1] = u.y; w[k][2] = u.z; w[k][3] = u.w; }
+        else if constexpr (V == 8) { const uint2 u = *reinterpret_cast<const uint2 *>(src); w[k][0] = u.x; w[k][1] = u.y; }
+        else w[k][0] = *src;
+    }
+#pragma unroll
+    for (int k = 0; k < N; k++) {
+        if (slot[k] >= num_slots) {                      // the row of out keeps what it held
+            if (row[k] != 0xFFFFFFFFu && d[k] == 0) report_error(err, KERR_SLOT_RANGE);
+            continue;
         }
-        Chunk<T, V>::store(dst, x);
+        float x[V];
+        if constexpr (V == 1) {
+            x[0] = __half2float(__half(__nv_cvt_fp8_to_halfraw((uint8_t)w[k][0], __NV_E4M3))) * scale[k];
+        } else {
+#pragma unroll
+            for (int j = 0; j < V / 2; j++) {
+                const __half2 h(__nv_cvt_fp8x2_to_halfraw2((uint16_t)(w[k][j / 2] >> (16 * (j & 1))), __NV_E4M3));
+                const float2 f = __half22float2(h);
+                x[2 * j] = f.x * scale[k];
+                x[2 * j + 1] = f.y * scale[k];
+            }
+        }
+        store_row<T, V>(out + (size_t)row[k] * kv_dim + d[k], x);
     }
 }
 
@@ -236,8 +286,8 @@ template <typename T, int VEC> cudaError_t rope_write(RopeWrite p, int tokens, i
     const int rows = p.nq + p.nk + p.nv, rpc = RW_THREADS / lpr, most = (rows + rpc - 1) / rpc;
     const int want = (2 * sm_count + tokens - 1) / tokens;
     const dim3 grid((unsigned)tokens, (unsigned)(want < most ? want : most));
-    if (vec) return launch_dependent(rope_write_kernel<T, VEC, 1>, grid, dim3(RW_THREADS), 0, s, pdl, p);
-    return launch_dependent(rope_write_kernel<T, 1, 8>, grid, dim3(RW_THREADS), 0, s, pdl, p);
+    if (vec) return launch_dependent(rope_write_kernel<T, VEC, 1, 3>, grid, dim3(RW_THREADS), 0, s, pdl, p);
+    return launch_dependent(rope_write_kernel<T, 1, 4, 1>, grid, dim3(RW_THREADS), 0, s, pdl, p);
 }
 
 }  // namespace
@@ -252,14 +302,21 @@ cudaError_t launch_gather_quant(void *out, int dtype, const uint8_t *pool, const
                                 uint32_t kv_dim, uint32_t head_dim, uint32_t num_slots, uint32_t rows, uint32_t *err,
                                 cudaStream_t s, bool pdl) {
     if (rows == 0) return cudaSuccess;
-    const uint32_t vec = dtype == DT_BF16 ? 8 : 4;
-    const bool ok = head_dim % vec == 0;
+    const uint32_t vec = dtype == DT_BF16 ? 16 : 8;      // 32 bytes of output
+    const bool ok = head_dim % vec == 0 && (uintptr_t)out % 32 == 0;
     const size_t n = (size_t)(kv_dim / (ok ? vec : 1)) * rows;
-    const dim3 grid((unsigned)((n + 255) / 256));
-#define LLMRS_GATHER(T, V) launch_dependent(gather_quant_kernel<T, V>, grid, dim3(256), 0, s, pdl, (T *)out, pool, scales, \
-                                            indices, kv_dim, head_dim, num_slots, rows, err)
-    if (dtype == DT_BF16) return ok ? LLMRS_GATHER(__nv_bfloat16, 8) : LLMRS_GATHER(__nv_bfloat16, 1);
-    return ok ? LLMRS_GATHER(float, 4) : LLMRS_GATHER(float, 1);
+    constexpr int N = 4;
+    // four units a thread once that still leaves every SM its share of warps; one each below
+    const int per = n >= (size_t)4 * 256 * 148 * 4 ? N : 1;
+    const dim3 grid((unsigned)((n + 256 * per - 1) / (256 * per)));
+#define LLMRS_GATHER(T, V, K) launch_dependent(gather_quant_kernel<T, V, K>, grid, dim3(256), 0, s, pdl, (T *)out, pool, scales, \
+                                               indices, kv_dim, head_dim, num_slots, rows, err)
+    if (dtype == DT_BF16) {
+        if (!ok) return per == N ? LLMRS_GATHER(__nv_bfloat16, 1, N) : LLMRS_GATHER(__nv_bfloat16, 1, 1);
+        return per == N ? LLMRS_GATHER(__nv_bfloat16, 16, N) : LLMRS_GATHER(__nv_bfloat16, 16, 1);
+    }
+    if (!ok) return per == N ? LLMRS_GATHER(float, 1, N) : LLMRS_GATHER(float, 1, 1);
+    return per == N ? LLMRS_GATHER(float, 8, N) : LLMRS_GATHER(float, 8, 1);
 #undef LLMRS_GATHER
 }
 

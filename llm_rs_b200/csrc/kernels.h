@@ -124,7 +124,7 @@ struct RopeWrite {
     uint32_t num_slots;
     float magnitude;
     int nq, nk, nv, head_dim, rotary, split_half;
-    int lanes_per_row;               // set by the launcher
+    int lanes_per_row, tokens, tokens_per_cta;       // set by the launcher
 };
 cudaError_t launch_rope_write(const RopeWrite &p, int dtype, int tokens, int sm_count, cudaStream_t s, bool pdl);
 // out[c] (F32 or BF16) = codes * scales of slot indices[c], c < rows.

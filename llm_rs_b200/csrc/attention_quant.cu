@@ -8,6 +8,8 @@
 // A row that sees nothing yields zeros.  Tokens behind the last request are left as they were.
 #include <cuda_fp8.h>
 
+#include <type_traits>
+
 #include "kernels.h"
 #include "llmrs_common.cuh"
 #include "pipeline.cuh"
@@ -1107,92 +1109,93 @@ attention_quant_long_kernel(const AttnQuant p, int skip_short, uint32_t polls) {
                     const uint32_t there = *reinterpret_cast<const uint32_t *>(sc + Sm::MASK + 4 * c);
                     return n <= 0 ? 0u : n >= 32 ? there : there & ((1u << n) - 1);
                 };
-                // ---- the row's maximum ----
-                float mx0 = -INFINITY, mx1 = -INFINITY;
-#pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    uint32_t v[32];
-                    tmem_ld32(s_col + 32 * c, v);
+                // Two forms of the code, chosen by the warp: most tiles are seen by every row whole, and a test a score costs
+                // more than the score's own arithmetic.  Each chunk of 32 columns is asked for while the one before is worked on.
+                auto work = [&](auto mask_tag) {
+                    constexpr bool MASKED = decltype(mask_tag)::value;
+                    uint32_t v[2][32];
+                    // ---- the row's maximum ----
+                    float mx0 = -INFINITY, mx1 = -INFINITY;
+                    tmem_ld32(s_col, v[0]);
                     tmem_ld_wait();
-                    if (!masked) {
+#pragma unroll
+                    for (int c = 0; c < 4; c++) {
+                        const uint32_t(&u)[32] = v[c & 1];
+                        tmem_ld32(s_col + 32 * ((c + 1) & 3), v[(c + 1) & 1]);           // after the last one the first again, for the weights
+                        uint32_t bits = 0;
+                        if constexpr (MASKED) bits = bits_of(c);
 #pragma unroll
                         for (int x = 0; x < 32; x += 4) {
                             const float4 k4 = *reinterpret_cast<const float4 *>(ks + 32 * c + x);
-                            const float2 a = pair_mul(make_float2(__uint_as_float(v[x]), __uint_as_float(v[x + 1])), make_float2(k4.x, k4.y));
-                            const float2 b = pair_mul(make_float2(__uint_as_float(v[x + 2]), __uint_as_float(v[x + 3])), make_float2(k4.z, k4.w));
+                            float2 a = pair_mul(make_float2(__uint_as_float(u[x]), __uint_as_float(u[x + 1])), make_float2(k4.x, k4.y));
+                            float2 d = pair_mul(make_float2(__uint_as_float(u[x + 2]), __uint_as_float(u[x + 3])), make_float2(k4.z, k4.w));
+                            if constexpr (MASKED) {
+                                if (!(bits >> x & 1)) a.x = -INFINITY;
+                                if (!(bits >> (x + 1) & 1)) a.y = -INFINITY;
+                                if (!(bits >> (x + 2) & 1)) d.x = -INFINITY;
+                                if (!(bits >> (x + 3) & 1)) d.y = -INFINITY;
+                            }
                             mx0 = fmaxf(mx0, fmaxf(a.x, a.y));
-                            mx1 = fmaxf(mx1, fmaxf(b.x, b.y));
+                            mx1 = fmaxf(mx1, fmaxf(d.x, d.y));
                         }
-                    } else {
-                        const uint32_t bits = bits_of(c);
-#pragma unroll
-                        for (int x = 0; x < 32; x++) {
-                            const float a = __uint_as_float(v[x]) * ks[32 * c + x];
-                            mx0 = fmaxf(mx0, bits >> x & 1 ? a : -INFINITY);
-                        }
-                    }
-                }
-                const float mx = fmaxf(mx0, mx1) * c_row;
-                // ---- move the reference, O and the sum where the maximum has outgrown it ----
-                const float m_new = mx > m_ref + LG_SLACK ? mx : m_ref;          // m_ref = -inf: any score at all
-                const bool moved = m_new != m_ref || r_new != r_bits;
-                const float base = m_new == -INFINITY ? 0.0f : m_new;
-                if (j > 0 && __any_sync(0xffffffffu, moved)) {
-                    const float f = m_new == m_ref ? 1.0f : ex2(m_ref - base);
-                    const float sh = r_new - r_bits >= (127u << 23) ? 0.0f : __uint_as_float(r_bits - r_new + (127u << 23));  // R / R'
-                    l2.x *= f;
-                    l2.y *= f;
-#pragma unroll
-                    for (int c = 0; c < HD / 32; c++) {
-                        uint32_t v[32];
-                        tmem_ld32(o_col + 32 * c, v);
                         tmem_ld_wait();
-                        uint32_t a[16], b[16];
-#pragma unroll
-                        for (int x = 0; x < 16; x++) {
-                            a[x] = __float_as_uint(__uint_as_float(v[x]) * (f * sh));
-                            b[x] = __float_as_uint(__uint_as_float(v[16 + x]) * (f * sh));
-                        }
-                        tmem_st16(o_col + 32 * c, a);
-                        tmem_st16(o_col + 32 * c + 16, b);
                     }
-                }
-                m_ref = m_new;
-                r_bits = r_new;
-                // ---- the weights, over the scores ----
-                const float2 c2 = make_float2(c_row, c_row), nb = make_float2(-base, -base);
+                    const float mx = fmaxf(mx0, mx1) * c_row;
+                    // ---- move the reference, O and the sum where the maximum has outgrown it ----
+                    const float m_new = mx > m_ref + LG_SLACK ? mx : m_ref;      // m_ref = -inf: any score at all
+                    const bool moved = m_new != m_ref || r_new != r_bits;
+                    const float base = m_new == -INFINITY ? 0.0f : m_new;
+                    if (j > 0 && __any_sync(0xffffffffu, moved)) {
+                        const float f = m_new == m_ref ? 1.0f : ex2(m_ref - base);
+                        const float sh = r_new - r_bits >= (127u << 23) ? 0.0f : __uint_as_float(r_bits - r_new + (127u << 23));      // R / R'
+                        l2.x *= f;
+                        l2.y *= f;
 #pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    uint32_t v[32], w[16];
-                    tmem_ld32(s_col + 32 * c, v);
-                    tmem_ld_wait();
-                    const uint32_t bits = masked ? bits_of(c) : 0xFFFFFFFFu;
+                        for (int c = 0; c < HD / 16; c++) {
+                            uint32_t o[16];
+                            tmem_ld16(o_col + 16 * c, o);
+                            tmem_ld_wait();
 #pragma unroll
-                    for (int x = 0; x < 32; x += 4) {
-                        const float4 k4 = *reinterpret_cast<const float4 *>(ks + 32 * c + x), w4 = *reinterpret_cast<const float4 *>(vw + 32 * c + x);
-#pragma unroll
-                        for (int y = 0; y < 2; y++) {
-                            const float2 k2 = y ? make_float2(k4.z, k4.w) : make_float2(k4.x, k4.y);
-                            const float2 w2 = y ? make_float2(w4.z, w4.w) : make_float2(w4.x, w4.y);
-                            const int at = x + 2 * y;
-                            float2 e = pair_op(pair_mul(make_float2(__uint_as_float(v[at]), __uint_as_float(v[at + 1])), k2), c2, nb);
-                            e.x = ex2(e.x);
-                            e.y = ex2(e.y);
-                            if (masked) {
-                                if (!(bits >> at & 1)) e.x = 0.0f;
-                                if (!(bits >> (at + 1) & 1)) e.y = 0.0f;
-                            }
-                            l2 = pair_add(l2, e);
-                            e = pair_mul(e, w2);
-                            if (masked) {                // not 0 * NaN
-                                if (!(bits >> at & 1)) e.x = 0.0f;
-                                if (!(bits >> (at + 1) & 1)) e.y = 0.0f;
-                            }
-                            w[at / 2] = pack_f16(e.x, e.y);
+                            for (int x = 0; x < 16; x++) o[x] = __float_as_uint(__uint_as_float(o[x]) * (f * sh));
+                            tmem_st16(o_col + 16 * c, o);
                         }
                     }
-                    tmem_st16(s_col + 16 * c, w);
-                }
+                    m_ref = m_new;
+                    r_bits = r_new;
+                    // ---- the weights, over the scores ----
+                    const float2 c2 = make_float2(c_row, c_row), nb = make_float2(-base, -base);
+#pragma unroll
+                    for (int c = 0; c < 4; c++) {
+                        const uint32_t(&u)[32] = v[c & 1];
+                        if (c < 3) tmem_ld32(s_col + 32 * (c + 1), v[(c + 1) & 1]);
+                        uint32_t bits = 0, w[16];
+                        if constexpr (MASKED) bits = bits_of(c);
+#pragma unroll
+                        for (int x = 0; x < 32; x += 4) {
+                            const float4 k4 = *reinterpret_cast<const float4 *>(ks + 32 * c + x), w4 = *reinterpret_cast<const float4 *>(vw + 32 * c + x);
+#pragma unroll
+                            for (int y = 0; y < 2; y++) {
+                                const float2 k2 = y ? make_float2(k4.z, k4.w) : make_float2(k4.x, k4.y);
+                                const float2 w2 = y ? make_float2(w4.z, w4.w) : make_float2(w4.x, w4.y);
+                                const int at = x + 2 * y;
+                                float2 e = pair_op(pair_mul(make_float2(__uint_as_float(u[at]), __uint_as_float(u[at + 1])), k2), c2, nb);
+                                e.x = ex2(e.x);
+                                e.y = ex2(e.y);
+                                float2 z = pair_mul(e, w2);
+                                if constexpr (MASKED) {              // the weight, too: 0 * NaN is not 0
+                                    if (!(bits >> at & 1)) e.x = z.x = 0.0f;
+                                    if (!(bits >> (at + 1) & 1)) e.y = z.y = 0.0f;
+                                }
+                                l2 = pair_add(l2, e);
+                                w[at / 2] = pack_f16(z.x, z.y);
+                            }
+                        }
+                        if (c < 3) tmem_ld_wait();
+                        tmem_st16(s_col + 16 * c, w);
+                    }
+                };
+                if (masked) work(std::true_type{});
+                else work(std::false_type{});
                 tmem_st_wait();
                 tc_fence_before();
                 mbar_arrive(&p_full[t]);

@@ -902,23 +902,36 @@ attention_quant_short_kernel(const __grid_constant__ ShortMaps maps, const AttnQ
 // SM's 16 a cycle.  So a CTA keeps two tiles of 128 query rows (token x head of the group, packed) against one
 // stream of keys and values: while one tile's weights are formed the tensor cores work for the other.
 //
-//   warps 0-3, 4-7   weights of tile 0, 1: a thread owns a row.  Scores come from TMEM 32 columns at a time, once for the
-//                    maximum and once for the weights, which go back as f16 over the scores that they came from.
-//   warps 8-11       keys and values: codes from memory to registers, one tile ahead, to f16 (exact), to shared memory in
-//                    the 128-byte swizzle; the scales, ready for use.  Any page size: rows are looked up one by one.
-//   warp 12          issues the products: S = Q K^T (both from shared memory), O += W V (W from TMEM; the values lie
+//   warps 0-3, 4-7   weights of tile 0, 1: a thread owns a row.  Scores come from TMEM 16 columns at a time, weights go back
+//                    as f16 over the scores that they came from.
+//   warps 8-11, 12-15   keys, values: codes to shared memory as they are, one tile ahead, then to f16 in the 128-byte
+//                    swizzle, the scales multiplied in.  Any page size: rows are looked up one by one.
+//   warp 16          issues the products: S = Q K^T (both from shared memory), O += W V (W from TMEM; the values lie
 //                    as they come, positions in rows, so they are the operand's major dimension the other way round).
 //
-// Softmax in one pass: O and the sum refer to a maximum that is only moved when a row's grows by more than 2 (log2), so O
-// is rarely rescaled; weights then stay below 4, and enter as e^(s - m) vs / R * 2^13 (R as in the other kernel).
-constexpr int LG_ROWS = 128, LG_POS = 128, LG_THREADS = 13 * 32;
-constexpr float LG_SLACK = 2.0f;     // log2: the weights' factor 2^13 leaves two octaves to f16's 65504
+// Softmax in one pass: O and the sum refer to a maximum that is only moved when a row's grows by more than 6 (log2), so O
+// is rarely rescaled (2 instead of 6: 4096 tokens 207 us instead of 191); weights then stay below 64, and enter as
+// e^(s - m) * 2^9: f16 keeps 2^-11 of a weight, and down to 2^-34 of the largest.
+//
+// The scales are multiplied into the f16 keys and values as these are made, once a code instead of once a score (scales
+// at the scores: 227 us): a key is code * ks / (least power of two that no ks of its tile exceeds) * 2^6, a value code * vs / R
+// * 2^6 (R as in the other kernel).  The product is rounded to f16, 2^-11 of itself at most; a key's ks enters as two f16, so
+// that nothing common to a whole score is rounded; a value's as one, 2^-11 more of a weight.  Scales below 2^-20 of
+// the power lose further bits: a value is kept to 2^-30 of the largest before it.  A value whose scale is not finite is
+// zero there, and the rows that see it are marked, so that no row sees NaN times zero.
+//
+// 128 query rows a tile, 4096 tokens of 32 heads over 8: 0.7 PFLOP/s; 1152 tokens behind 31616: 1.0 (59 % of measured).  What
+// is left there is the issue of the weights' 3.5 instructions a score and, for short prompts, a CTA's start and end
+// (about 8 us: lookups, queries, first keys; one CTA fits an SM).
+constexpr int LG_ROWS = 128, LG_POS = 128, LG_THREADS = 17 * 32;
+constexpr float LG_SLACK = 6.0f;     // log2: the weights' factor 2^9 leaves these octaves to f16's 65504
 
 template <int HD> struct LongSmem {
     static constexpr int HALVES = HD / 64, TILE = LG_ROWS * HD * 2;      // 128 rows of f16, in halves of 64 dimensions
-    static constexpr int Q = 0, K = 2 * TILE, V = K + 2 * TILE, SC = V + 2 * TILE;
-    // scales of a tile of positions: ks [128], vs / R * 2^13 [128], which positions are there [4], all there, R's bits
-    static constexpr int STAGES = 3, KS = 0, VW = 512, MASK = 1024, ALL = 1040, RBITS = 1044, SCALES = 1152;
+    static constexpr int Q = 0, K = 2 * TILE, V = K + 2 * TILE, RAW = V + 2 * TILE, SC = RAW + 2 * (TILE / 2);
+    // of a tile of positions: which are there [4], whose value's scale is not finite [4], whether nothing of this needs a
+    // look, R's bits, the factor of its scores
+    static constexpr int STAGES = 3, MASK = 0, BAD = 16, ALL = 32, RBITS = 36, KREF = 40, SCALES = 64;
     static constexpr int BYTES = SC + STAGES * SCALES;
 };
 
@@ -985,7 +998,7 @@ attention_quant_long_kernel(const AttnQuant p, int skip_short, uint32_t polls) {
     constexpr int CH = HD / 16;                          // 16-byte chunks of codes in a row
     extern __shared__ __align__(1024) uint8_t lg_smem[];
     __shared__ __align__(8) uint64_t q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], sc_full[Sm::STAGES], sc_empty[Sm::STAGES], s_full[2], p_full[2], o_full[2];
-    __shared__ uint32_t tmem_base_s, vmax_s[2][4], gone_s[2][4];
+    __shared__ uint32_t tmem_base_s, top_s[2][2][4], look_s[2][4];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if (tid == 0) {
         for (int i = 0; i < 2; i++) {
@@ -999,7 +1012,7 @@ attention_quant_long_kernel(const AttnQuant p, int skip_short, uint32_t polls) {
             mbar_init(&o_full[i], 1);
         }
         for (int i = 0; i < Sm::STAGES; i++) {
-            mbar_init(&sc_full[i], 128);
+            mbar_init(&sc_full[i], 256);
             mbar_init(&sc_empty[i], 8);
         }
         mbar_init_fence();
@@ -1047,7 +1060,7 @@ attention_quant_long_kernel(const AttnQuant p, int skip_short, uint32_t polls) {
     }
     const int n_tiles = max(nt[0], nt[1]);               // tile 1's rows come later and see more, if there are any
     const int kv_end = r.before + (row0 + min(rows, 2 * LG_ROWS) - 1) / group + 1;
-    if (warp == 12) { tmem_alloc(&tmem_base_s, 512); tmem_relinquish(); }
+    if (warp == 16) { tmem_alloc(&tmem_base_s, 512); tmem_relinquish(); }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -1068,7 +1081,7 @@ attention_quant_long_kernel(const AttnQuant p, int skip_short, uint32_t polls) {
         // the row of queries: its size, then scaled by a power of two to f16 and into the operand's layout
         float amax = 0.0f;
         const uint16_t *q = (const uint16_t *)p.q + off;
-#pragma unroll 4
+#pragma unroll 8
         for (int c = 0; c < HD / 8; c++) {
             const uint4 u = on ? *reinterpret_cast<const uint4 *>(q + 8 * c) : make_uint4(0, 0, 0, 0);
             const uint32_t w[4] = {u.x, u.y, u.z, u.w};
@@ -1077,7 +1090,7 @@ attention_quant_long_kernel(const AttnQuant p, int skip_short, uint32_t polls) {
         }
         const int ex = row_exponent(amax);
         const float up = exp2i(ex), c_row = exp2i(-ex) * (1.4426950408889634f / sqrtf((float)HD));
-#pragma unroll 4
+#pragma unroll 8
         for (int c = 0; c < HD / 8; c++) {
             const uint4 u = on ? *reinterpret_cast<const uint4 *>(q + 8 * c) : make_uint4(0, 0, 0, 0);
             const uint32_t w[4] = {u.x, u.y, u.z, u.w};
@@ -1099,7 +1112,7 @@ attention_quant_long_kernel(const AttnQuant p, int skip_short, uint32_t polls) {
             wait(&sc_full[st], (j / Sm::STAGES) & 1, KERR_FULL_WAIT);
             if (j < nt[t]) {
                 const uint8_t *sc = lg_smem + Sm::SC + st * Sm::SCALES;
-                const float *ks = reinterpret_cast<const float *>(sc + Sm::KS), *vw = reinterpret_cast<const float *>(sc + Sm::VW);
+                const float c_tile = c_row * *reinterpret_cast<const float *>(sc + Sm::KREF);
                 const uint32_t r_new = *reinterpret_cast<const uint32_t *>(sc + Sm::RBITS);
                 const bool masked = !full_tile || (j + 1) * LG_POS > min_len || *reinterpret_cast<const uint32_t *>(sc + Sm::ALL) == 0;
                 wait(&s_full[t], j & 1, KERR_MMA_WAIT);
@@ -1110,37 +1123,35 @@ attention_quant_long_kernel(const AttnQuant p, int skip_short, uint32_t polls) {
                     return n <= 0 ? 0u : n >= 32 ? there : there & ((1u << n) - 1);
                 };
                 // Two forms of the code, chosen by the warp: most tiles are seen by every row whole, and a test a score costs
-                // more than the score's own arithmetic.  Each chunk of 32 columns is asked for while the one before is worked on.
+                // more than the score's own arithmetic.  Each 16 columns are asked for while the 16 before are worked on.
                 auto work = [&](auto mask_tag) {
                     constexpr bool MASKED = decltype(mask_tag)::value;
-                    uint32_t v[2][32];
+                    uint32_t v[2][16];
                     // ---- the row's maximum ----
                     float mx0 = -INFINITY, mx1 = -INFINITY;
-                    tmem_ld32(s_col, v[0]);
+                    tmem_ld16(s_col, v[0]);
                     tmem_ld_wait();
 #pragma unroll
-                    for (int c = 0; c < 4; c++) {
-                        const uint32_t(&u)[32] = v[c & 1];
-                        tmem_ld32(s_col + 32 * ((c + 1) & 3), v[(c + 1) & 1]);           // after the last one the first again, for the weights
+                    for (int c = 0; c < 8; c++) {
+                        const uint32_t(&u)[16] = v[c & 1];
+                        tmem_ld16(s_col + 16 * ((c + 1) & 7), v[(c + 1) & 1]);           // after the last one the first again, for the weights
                         uint32_t bits = 0;
-                        if constexpr (MASKED) bits = bits_of(c);
+                        if constexpr (MASKED) bits = bits_of(c >> 1) >> (16 * (c & 1));
 #pragma unroll
-                        for (int x = 0; x < 32; x += 4) {
-                            const float4 k4 = *reinterpret_cast<const float4 *>(ks + 32 * c + x);
-                            float2 a = pair_mul(make_float2(__uint_as_float(u[x]), __uint_as_float(u[x + 1])), make_float2(k4.x, k4.y));
-                            float2 d = pair_mul(make_float2(__uint_as_float(u[x + 2]), __uint_as_float(u[x + 3])), make_float2(k4.z, k4.w));
-                            if constexpr (MASKED) {
-                                if (!(bits >> x & 1)) a.x = -INFINITY;
-                                if (!(bits >> (x + 1) & 1)) a.y = -INFINITY;
-                                if (!(bits >> (x + 2) & 1)) d.x = -INFINITY;
-                                if (!(bits >> (x + 3) & 1)) d.y = -INFINITY;
+                        for (int x = 0; x < 16; x += 4) {
+                            float a[4];
+#pragma unroll
+                            for (int y = 0; y < 4; y++) {
+                                a[y] = __uint_as_float(u[x + y]);
+                                if constexpr (MASKED)
+                                    if (!(bits >> (x + y) & 1)) a[y] = -INFINITY;
                             }
-                            mx0 = fmaxf(mx0, fmaxf(a.x, a.y));
-                            mx1 = fmaxf(mx1, fmaxf(d.x, d.y));
+                            mx0 = fmaxf(mx0, fmaxf(a[0], a[1]));
+                            mx1 = fmaxf(mx1, fmaxf(a[2], a[3]));
                         }
                         tmem_ld_wait();
                     }
-                    const float mx = fmaxf(mx0, mx1) * c_row;
+                    const float mx = fmaxf(mx0, mx1) * c_tile;
                     // ---- move the reference, O and the sum where the maximum has outgrown it ----
                     const float m_new = mx > m_ref + LG_SLACK ? mx : m_ref;      // m_ref = -inf: any score at all
                     const bool moved = m_new != m_ref || r_new != r_bits;
@@ -1163,36 +1174,36 @@ attention_quant_long_kernel(const AttnQuant p, int skip_short, uint32_t polls) {
                     m_ref = m_new;
                     r_bits = r_new;
                     // ---- the weights, over the scores ----
-                    const float2 c2 = make_float2(c_row, c_row), nb = make_float2(-base, -base);
+                    const float2 c2 = make_float2(c_tile, c_tile), nb = make_float2(9.0f - base, 9.0f - base);
+                    bool bad = false;
 #pragma unroll
-                    for (int c = 0; c < 4; c++) {
-                        const uint32_t(&u)[32] = v[c & 1];
-                        if (c < 3) tmem_ld32(s_col + 32 * (c + 1), v[(c + 1) & 1]);
-                        uint32_t bits = 0, w[16];
-                        if constexpr (MASKED) bits = bits_of(c);
+                    uint32_t w[16];
 #pragma unroll
-                        for (int x = 0; x < 32; x += 4) {
-                            const float4 k4 = *reinterpret_cast<const float4 *>(ks + 32 * c + x), w4 = *reinterpret_cast<const float4 *>(vw + 32 * c + x);
-#pragma unroll
-                            for (int y = 0; y < 2; y++) {
-                                const float2 k2 = y ? make_float2(k4.z, k4.w) : make_float2(k4.x, k4.y);
-                                const float2 w2 = y ? make_float2(w4.z, w4.w) : make_float2(w4.x, w4.y);
-                                const int at = x + 2 * y;
-                                float2 e = pair_op(pair_mul(make_float2(__uint_as_float(u[at]), __uint_as_float(u[at + 1])), k2), c2, nb);
-                                e.x = ex2(e.x);
-                                e.y = ex2(e.y);
-                                float2 z = pair_mul(e, w2);
-                                if constexpr (MASKED) {              // the weight, too: 0 * NaN is not 0
-                                    if (!(bits >> at & 1)) e.x = z.x = 0.0f;
-                                    if (!(bits >> (at + 1) & 1)) e.y = z.y = 0.0f;
-                                }
-                                l2 = pair_add(l2, e);
-                                w[at / 2] = pack_f16(z.x, z.y);
-                            }
+                    for (int c = 0; c < 8; c++) {
+                        const uint32_t(&u)[16] = v[c & 1];
+                        if (c < 7) tmem_ld16(s_col + 16 * (c + 1), v[(c + 1) & 1]);
+                        uint32_t bits = 0;
+                        if constexpr (MASKED) {
+                            bits = bits_of(c >> 1);
+                            bad = bad || (bits & *reinterpret_cast<const uint32_t *>(sc + Sm::BAD + 4 * (c >> 1))) != 0;
+                            bits >>= 16 * (c & 1);
                         }
-                        if (c < 3) tmem_ld_wait();
-                        tmem_st16(s_col + 16 * c, w);
+#pragma unroll
+                        for (int x = 0; x < 16; x += 2) {
+                            float2 e = pair_op(make_float2(__uint_as_float(u[x]), __uint_as_float(u[x + 1])), c2, nb);
+                            e.x = ex2(e.x);
+                            e.y = ex2(e.y);
+                            if constexpr (MASKED) {
+                                if (!(bits >> x & 1)) e.x = 0.0f;
+                                if (!(bits >> (x + 1) & 1)) e.y = 0.0f;
+                            }
+                            l2 = pair_add(l2, e);
+                            w[8 * (c & 1) + x / 2] = pack_f16(e.x, e.y);
+                        }
+                        if (c < 7) tmem_ld_wait();
+                        if (c & 1) tmem_st16(s_col + 16 * (c >> 1), w);
                     }
+                    if (MASKED && bad) l2.x = __int_as_float(0x7FC00000);        // sees a value that is NaN
                 };
                 if (masked) work(std::true_type{});
                 else work(std::false_type{});
@@ -1205,7 +1216,7 @@ attention_quant_long_kernel(const AttnQuant p, int skip_short, uint32_t polls) {
         }
         // ---- O, divided by the sum ----
         const float l = l2.x + l2.y;
-        const float norm = l == 0.0f ? 0.0f : __uint_as_float(r_bits - (13u << 23)) / l;
+        const float norm = l == 0.0f ? 0.0f : __uint_as_float(r_bits - (6u << 23)) / l;
         uint16_t *out = (uint16_t *)p.out + off;
         if (nt[t] > 0) {
             wait(&o_full[t], 0, KERR_MMA_WAIT);
@@ -1233,91 +1244,111 @@ attention_quant_long_kernel(const AttnQuant p, int skip_short, uint32_t polls) {
             }
         }
         tc_fence_before();
-    } else if (warp < 12) {
-        // ================= keys and values =================
-        const int w = warp - 8;                          // this warp's positions are 32 w .. 32 w + 31 of a tile
+    } else if (warp < 16) {
+        // ================= keys (warps 8-11), values (12-15) =================
+        const bool keys = warp < 12;
+        const int w = warp & 3;                          // this warp's positions are 32 w .. 32 w + 31 of a tile
         const size_t kv_dim = (size_t)p.n_kv * HD;
         const uint32_t *table = p.block_table + (size_t)req * p.max_blocks;
-        const uint8_t *kp = p.k_pool + (size_t)kvh * HD, *vp = p.v_pool + (size_t)kvh * HD;
-        const float *ksp = p.k_scales + (size_t)kvh * p.num_slots, *vsp = p.v_scales + (size_t)kvh * p.num_slots;
+        const uint8_t *pool = (keys ? p.k_pool : p.v_pool) + (size_t)kvh * HD;
+        const float *scales = (keys ? p.k_scales : p.v_scales) + (size_t)kvh * p.num_slots;
         constexpr int RPI = 32 / CH, N = 32 / RPI;       // rows a pass, passes
         const int c = lane % CH;
-        uint4 kr[N], vr[N];
-        float ks = 0.0f, vs = 0.0f;
-        uint32_t there = 0, page = 0;
+        uint64_t *full = keys ? k_full : v_full, *empty = keys ? k_empty : v_empty;
+        uint8_t *tiles = lg_smem + (keys ? Sm::K : Sm::V), *raw = lg_smem + Sm::RAW + (keys ? 0 : Sm::TILE / 2) + w * 32 * HD;
+        float scale_next = 0.0f;
+        uint32_t there_next = 0, page = 0;
         auto page_of = [&](int j) -> uint32_t {
             const int pos = j * LG_POS + 32 * w + lane;
             return pos < kv_end ? table[pos / p.block_size] : 0u;
         };
-        auto load = [&](int j) {                         // the codes and scales of tile j, and the page of the tile after it
+        // The codes travel to shared memory as they are, a tile ahead; the thread that asked for 16 of them converts them, so
+        // nobody else waits for them.  Lane x looks up position 32 w + x, and has its scale.
+        auto ask = [&](int j) {
             const int pos = j * LG_POS + 32 * w + lane;
             const unsigned long long s64 = (unsigned long long)page * p.block_size + (unsigned)(pos % p.block_size);
             const bool ok = pos < kv_end && s64 < p.num_slots;
             if (pos < kv_end && !ok) report_error(p.err, KERR_SLOT_RANGE);
             const uint32_t slot = ok ? (uint32_t)s64 : 0u;
-            there = __ballot_sync(0xffffffffu, ok);
-            ks = ok ? __ldg(ksp + slot) : 0.0f;
-            vs = ok ? __ldg(vsp + slot) : 0.0f;
+            there_next = __ballot_sync(0xffffffffu, ok);
+            scale_next = ok ? __ldg(scales + slot) : 0.0f;
 #pragma unroll
             for (int x = 0; x < N; x++) {
                 const int row = x * RPI + lane / CH;
                 const size_t at = (size_t)__shfl_sync(0xffffffffu, slot, row) * kv_dim + 16 * c;
-                const bool on = there >> row & 1;
-                kr[x] = on ? ldg128(kp + at) : make_uint4(0, 0, 0, 0);
-                vr[x] = on ? ldg128(vp + at) : make_uint4(0, 0, 0, 0);
+                copy16_or_zero(raw + row * HD + 16 * c, pool + at, there_next >> row & 1);
             }
+            asm volatile("cp.async.commit_group;" ::: "memory");
             page = page_of(j + 1);
         };
-        auto store = [&](uint8_t *tile, const uint4 (&raw)[N]) {
-#pragma unroll
-            for (int x = 0; x < N; x++) {
-                const int row = 32 * w + x * RPI + lane / CH;
-                uint32_t h[8];
-                codes_to_f16(raw[x].x, h[0], h[1]);
-                codes_to_f16(raw[x].y, h[2], h[3]);
-                codes_to_f16(raw[x].z, h[4], h[5]);
-                codes_to_f16(raw[x].w, h[6], h[7]);
-                *reinterpret_cast<uint4 *>(tile + f16_chunk_at(row, 2 * c)) = make_uint4(h[0], h[1], h[2], h[3]);
-                *reinterpret_cast<uint4 *>(tile + f16_chunk_at(row, 2 * c + 1)) = make_uint4(h[4], h[5], h[6], h[7]);
-            }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        };
-        uint32_t r_bits = 17u << 23;
+        auto power_above = [](uint32_t bits) { return min((bits + 0x7FFFFFu) & 0x7F800000u, 253u << 23); };      // of two
+        uint32_t power = 17u << 23;                      // values: R, which only grows; keys: of the tile
         if (n_tiles > 0) {
             page = page_of(0);
-            load(0);
+            ask(0);
         }
         for (int j = 0; j < n_tiles; j++) {
             const int b = j & 1, st = j % Sm::STAGES;
-            const uint32_t par = ((j >> 1) & 1) ^ 1;
-            // scales, with R the least power of two that no vs so far exceeds
-            float vmax = fmaxf(0.0f, vs);
+            const uint32_t there = there_next;
+            const bool ok = keys || scale_next <= 3.402823466e38f;       // a value's scale that is NaN or infinite: zeros, and marked
+            const float scale = ok ? scale_next : 0.0f;
+            float top = fmaxf(0.0f, scale);
 #pragma unroll
-            for (int o = 16; o; o >>= 1) vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, o));
+            for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            const uint32_t bad = __ballot_sync(0xffffffffu, !ok);
             if (lane == 0) {
-                vmax_s[b][w] = __float_as_uint(vmax);
-                gone_s[b][w] = there != 0xFFFFFFFFu;     // positions past kv_end, or on a page beyond the pool
+                top_s[keys][b][w] = __float_as_uint(top);
+                if (!keys) look_s[b][w] = there != 0xFFFFFFFFu || bad;   // positions past kv_end, on a page beyond the pool, or marked
             }
-            if (j >= 2) wait(&k_empty[b], par, KERR_EMPTY_WAIT);
-            store(lg_smem + Sm::K + b * Sm::TILE, kr);
-            mbar_arrive(&k_full[b]);
+            named_barrier_sync(keys ? 2 : 3, 128);       // what the four warps have found
+            const uint32_t *tops = top_s[keys][b];
+            const uint32_t above = power_above(max(max(tops[0], tops[1]), max(tops[2], tops[3])));
+            power = max(keys ? 17u << 23 : power, above);
             if (j >= Sm::STAGES) wait(&sc_empty[st], ((j / Sm::STAGES) & 1) ^ 1, KERR_EMPTY_WAIT);
-            named_barrier_sync(2, 128);                  // what the four warps have found
-            const uint32_t top = max(max(vmax_s[b][0], vmax_s[b][1]), max(vmax_s[b][2], vmax_s[b][3]));
-            r_bits = max(r_bits, min((top + 0x7FFFFFu) & 0x7F800000u, 253u << 23));
             uint8_t *sc = lg_smem + Sm::SC + st * Sm::SCALES;
-            reinterpret_cast<float *>(sc + Sm::KS)[32 * w + lane] = ks;
-            reinterpret_cast<float *>(sc + Sm::VW)[32 * w + lane] = vs * __uint_as_float(((127u + 127u + 13u) << 23) - r_bits);       // 2^13 / R
-            if (lane == 0) reinterpret_cast<uint32_t *>(sc + Sm::MASK)[w] = there;
-            if (tid == 8 * 32) {
-                *reinterpret_cast<uint32_t *>(sc + Sm::ALL) = !(gone_s[b][0] | gone_s[b][1] | gone_s[b][2] | gone_s[b][3]);
-                *reinterpret_cast<uint32_t *>(sc + Sm::RBITS) = r_bits;
+            if (keys) {
+                if (lane == 0) reinterpret_cast<uint32_t *>(sc + Sm::MASK)[w] = there;
+                if (w == 0 && lane == 0) *reinterpret_cast<uint32_t *>(sc + Sm::KREF) = power - (6u << 23);
+            } else {
+                if (lane == 0) reinterpret_cast<uint32_t *>(sc + Sm::BAD)[w] = bad;
+                if (w == 0 && lane == 0) {
+                    *reinterpret_cast<uint32_t *>(sc + Sm::ALL) = !(look_s[b][0] | look_s[b][1] | look_s[b][2] | look_s[b][3]);
+                    *reinterpret_cast<uint32_t *>(sc + Sm::RBITS) = power;
+                }
             }
             mbar_arrive(&sc_full[st]);
-            if (j >= 2) wait(&v_empty[b], par, KERR_EMPTY_WAIT);
-            store(lg_smem + Sm::V + b * Sm::TILE, vr);
-            mbar_arrive(&v_full[b]);
-            if (j + 1 < n_tiles) load(j + 1);
+            // The scale over the power of two, times 2^6, as f16 hi + lo; a value does with hi, whose 2^-12 is one more rounding
+            // of a weight, a key's score would be off by as much of itself.
+            const float fs = scale * __uint_as_float(((127u + 127u + 6u) << 23) - power);
+            const __half hi = __float2half_rn(fs), lo = __float2half_rn(keys ? fs - __half2float(hi) : 0.0f);
+            const uint32_t pair = (uint32_t)__half_as_ushort(hi) | (uint32_t)__half_as_ushort(lo) << 16;
+            if (j >= 2) wait(&empty[b], ((j >> 1) & 1) ^ 1, KERR_EMPTY_WAIT);
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
+            uint8_t *tile = tiles + b * Sm::TILE;
+            auto convert = [&](auto key_tag) {
+#pragma unroll
+                for (int x = 0; x < N; x++) {
+                    const int row = x * RPI + lane / CH;
+                    const uint32_t f = __shfl_sync(0xffffffffu, pair, row), f_hi = h2_bcast_lo(f), f_lo = h2_bcast_hi(f);
+                    const uint4 u = *reinterpret_cast<const uint4 *>(raw + row * HD + 16 * c);
+                    const uint32_t r4[4] = {u.x, u.y, u.z, u.w};
+                    uint32_t h[8];
+#pragma unroll
+                    for (int y = 0; y < 4; y++) codes_to_f16(r4[y], h[2 * y], h[2 * y + 1]);
+#pragma unroll
+                    for (int y = 0; y < 8; y++) {
+                        if constexpr (decltype(key_tag)::value) h[y] = h2_fma(h[y], f_hi, h2_mul(h[y], f_lo));
+                        else h[y] = h2_mul(h[y], f_hi);
+                    }
+                    *reinterpret_cast<uint4 *>(tile + f16_chunk_at(32 * w + row, 2 * c)) = make_uint4(h[0], h[1], h[2], h[3]);
+                    *reinterpret_cast<uint4 *>(tile + f16_chunk_at(32 * w + row, 2 * c + 1)) = make_uint4(h[4], h[5], h[6], h[7]);
+                }
+            };
+            if (keys) convert(std::true_type{});
+            else convert(std::false_type{});
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            mbar_arrive(&full[b]);
+            if (j + 1 < n_tiles) ask(j + 1);
         }
     } else {
         // ================= products =================
@@ -1375,7 +1406,7 @@ attention_quant_long_kernel(const AttnQuant p, int skip_short, uint32_t polls) {
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 12) {
+    if (warp == 16) {
         tc_fence_after();
         tmem_dealloc(tmem, 512);
     }

@@ -157,8 +157,11 @@ __global__ void __launch_bounds__(AQ_TILE) attention_quant_simple_kernel(const A
 // sequence that is cut into equal contiguous ranges, one per CTA, so ragged batches load every SM alike and one
 // long request spreads over the whole GPU.  The lengths are on the device, so each CTA adds them up itself.  A row
 // block that lies in several ranges leaves (accumulator, maximum, sum) parts in the workspace; the last CTA to finish of
-// each 18 neighbours joins theirs, and the last of those the rest, always in the order of the parts (a second
-// kernel for it cost 5 us of 14 for one request of 1000 positions and 65 us beside 97 for 64 requests).
+// each 18 neighbours joins theirs, and the last of those the rest, always in the order of the parts (few requests:
+// attention_quant_merge_kernel).
+//
+// One request of 131071 positions: 57 us, 74 % of the measured HBM rate; without the joining 49 (86 %).  64 requests of
+// 100 to 8192: 108 us, 79 %; without 97 (88 %).
 //
 // A CTA has 8 consumer warps, HW heads x PW runs of 16 positions, so that neighbouring heads of a slot, neighbours
 // in memory, are read at the same time, and a producer that keeps NST units in flight, through to the end of the
@@ -468,7 +471,7 @@ __device__ __forceinline__ bool last_of(uint32_t *counter, uint32_t n, uint32_t 
 template <int HD, int RB, int TERMS, int HW, int NST, bool TMA>
 __global__ void __launch_bounds__(SH_THREADS + (TMA ? 32 : 128), 2)
 attention_quant_short_kernel(const __grid_constant__ ShortMaps maps, const AttnQuant p, int bf16, int only_short, uint32_t polls,
-                             float *__restrict__ ws, uint32_t *__restrict__ counters) {
+                             float *__restrict__ ws, uint32_t *__restrict__ counters, int join_here) {
     using St = ShortStage<HD, HW>;
     constexpr int PW = SH_WARPS / HW, RUNS = St::RUNS, TP = 16 * RUNS, KS = HD / 16, CH = HD / 16, NT = RB / 8;
     constexpr int PASS = 1;                              // chunks of 16 dimensions the warps of a head exchange at a time
@@ -875,7 +878,7 @@ attention_quant_short_kernel(const __grid_constant__ ShortMaps maps, const AttnQ
                 }
             }
         }
-        if (whole) continue;
+        if (whole || !join_here) continue;
         const int c0 = holder(total, n_cta, s.item), c1 = holder(total, n_cta, s.item + s.tiles - 1);
         const int g0 = cta / SH_JOIN * SH_JOIN, gf = max(c0, g0), gl = min(c1, g0 + SH_JOIN - 1);    // of these neighbours
         // a CTA's first part, or its second if the row block starts within its range, which only the first holder's can
@@ -1448,6 +1451,7 @@ size_t short_workspace(const AttnQuant &p, const ShortPlan &s, int sm_count) {
     return (size_t)short_grid(p, s, sm_count) * 2 * s.hw * s.rb * (p.head_dim + 2) * sizeof(float);
 }
 
+constexpr int MERGE_THREADS = 512, MERGE_REQUESTS = 8;       // of attention_quant_merge_kernel
 // What the launches of one call share.
 struct ShortCall {
     ShortMaps maps;
@@ -1457,6 +1461,7 @@ struct ShortCall {
     uint32_t *counters;
     bool tma, pdl;
     cudaStream_t stream;
+    uint64_t *launches;
 };
 // Runs of 16 positions stay within a page, and the scales of a KV head start on 16 bytes.
 bool tma_fits(const AttnQuant &p) { return p.block_size % 16 == 0 && p.num_slots % 4 == 0; }
@@ -1490,7 +1495,7 @@ cudaError_t launch_short(const AttnQuant &p, const ShortCall &c) {
     const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;
     return launch_dependent(k, dim3((unsigned)c.grid), dim3(SH_THREADS + (TMA ? 32 : 128)), smem, c.stream, c.pdl, c.maps, p,
-                            (int)(c.dtype == DT_BF16), c.only_short, c.polls, c.ws, c.counters);
+                            (int)(c.dtype == DT_BF16), c.only_short, c.polls, c.ws, c.counters, (int)(p.num_req > MERGE_REQUESTS));
 }
 template <int HD, int RB, int TERMS, int NST>
 cudaError_t launch_short_hw(const AttnQuant &p, int hw, const ShortCall &c) {
@@ -1500,11 +1505,89 @@ cudaError_t launch_short_hw(const AttnQuant &p, int hw, const ShortCall &c) {
         default: return c.tma ? launch_short<HD, RB, TERMS, 1, NST, true>(p, c) : launch_short<HD, RB, TERMS, 1, NST, false>(p, c);
     }
 }
+// The parts of one row (query token, head), joined in order: the form for few requests, each in many parts, where a CTA a
+// row has more loads under way than the CTAs that happen to be last (one request of 131071 positions, 148 parts a row: 57 us
+// in all instead of 67, one of 1000: 11.9 instead of 14.4).  Looking its request up costs a CTA too much where there are many
+// (64 requests: 65 us for this kernel beside 97), and there are few parts a row to join then.
+template <int HD>
+__global__ void __launch_bounds__(MERGE_THREADS)
+attention_quant_merge_kernel(const AttnQuant p, int bf16, const Rows rows, int ctas, const float *__restrict__ ws) {
+    constexpr int PER = MERGE_THREADS / (HD / 4);        // parts at a time: HD / 4 threads to one
+    __shared__ float4 acc_s[MERGE_THREADS];
+    __shared__ float red[MERGE_THREADS / 32], lsum[PER];
+    const int head = blockIdx.x % p.n_heads, gq = blockIdx.x / p.n_heads, tid = threadIdx.x;
+    const int group = p.n_heads / p.n_kv, kvh = head / group;
+    pdl_prologue();
+    Request r = {0, 0, 0};
+    int blocks = 0, tiles = 0;
+    long long total = 0, before = 0;
+#pragma unroll
+    for (int q = 0; q < MERGE_REQUESTS; q++) {
+        if (q >= p.num_req) break;
+        const Request x = request_of(p, q);
+        int b, t;
+        shape_of(p, rows, x, b, t);
+        if (gq >= x.first && gq < x.first + x.count) { r = x; blocks = b; tiles = t; before = total; }
+        total += (long long)b * t;
+    }
+    if (blocks == 0) return;                             // behind the last request, or the other kernel's
+    const int rr = (gq - r.first) * group + head % group, rb = rr / rows.rb, i = rr % rows.rb;
+    const int n = sharers(total, ctas), groups = p.n_kv / rows.hw, hg = kvh / rows.hw, hd = kvh % rows.hw;
+    const long long item = before + (long long)rb * tiles;
+    const int c0 = holder(total, n, item), c1 = holder(total, n, item + tiles - 1);
+    if (c0 == c1) return;                                // one CTA had all of it and wrote the row
+    const int inside = item > first_unit(total, n, c0) ? 1 : 0;
+    const float2 *ml = reinterpret_cast<const float2 *>(ws + (size_t)ctas * groups * 2 * rows.hw * rows.rb * HD);
+    auto part = [&](int c) { return ((size_t)((c * groups + hg) * 2 + (c == c0 ? inside : 0)) * rows.hw + hd) * rows.rb + i; };
+    float m = -INFINITY;
+    for (int c = c0 + tid; c <= c1; c += MERGE_THREADS) m = fmaxf(m, ml[part(c)].x);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if ((tid & 31) == 0) red[tid >> 5] = m;
+    __syncthreads();
+    m = red[0];
+#pragma unroll
+    for (int w = 1; w < MERGE_THREADS / 32; w++) m = fmaxf(m, red[w]);
+    const float base = m == -INFINITY ? 0.0f : m;
+    const int d = 4 * (tid % (HD / 4)), mine = tid / (HD / 4);
+    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    float l = 0.0f;
+#pragma unroll 4
+    for (int c = c0 + mine; c <= c1; c += PER) {
+        const size_t x = part(c);
+        const float2 v = ml[x];
+        const float4 q = *reinterpret_cast<const float4 *>(ws + x * HD + d);
+        const float w = ex2(v.x - base);
+        l = fmaf(v.y, w, l);
+        acc.x = fmaf(q.x, w, acc.x); acc.y = fmaf(q.y, w, acc.y); acc.z = fmaf(q.z, w, acc.z); acc.w = fmaf(q.w, w, acc.w);
+    }
+    acc_s[tid] = acc;
+    if (d == 0) lsum[mine] = l;
+    __syncthreads();
+    if (tid >= HD / 4) return;
+    l = 0.0f;
+    acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+    for (int x = 0; x < PER; x++) {
+        const float4 q = acc_s[x * (HD / 4) + tid];
+        l += lsum[x];
+        acc.x += q.x; acc.y += q.y; acc.z += q.z; acc.w += q.w;
+    }
+    const float norm = l == 0.0f ? 0.0f : 1.0f / l;
+    store4(p.out, ((size_t)gq * p.n_heads + head) * HD + d, make_float4(acc.x * norm, acc.y * norm, acc.z * norm, acc.w * norm), bf16);
+}
+
 template <int HD>
 cudaError_t launch_short_all(const AttnQuant &p, const ShortPlan &pl, const ShortCall &c) {
     constexpr int NST = HD == 128 ? 3 : 5;
-    if (pl.terms == 2) return pl.rb == 8 ? launch_short_hw<HD, 8, 2, NST>(p, pl.hw, c) : launch_short_hw<HD, 16, 2, NST>(p, pl.hw, c);
-    return pl.rb == 8 ? launch_short_hw<HD, 8, 1, NST>(p, pl.hw, c) : launch_short_hw<HD, 16, 1, NST>(p, pl.hw, c);
+    cudaError_t e;
+    if (pl.terms == 2) e = pl.rb == 8 ? launch_short_hw<HD, 8, 2, NST>(p, pl.hw, c) : launch_short_hw<HD, 16, 2, NST>(p, pl.hw, c);
+    else e = pl.rb == 8 ? launch_short_hw<HD, 8, 1, NST>(p, pl.hw, c) : launch_short_hw<HD, 16, 1, NST>(p, pl.hw, c);
+    if (e != cudaSuccess || p.num_req > MERGE_REQUESTS) return e;
+    const Rows rows{pl.rb, 16 * SH_TILES / pl.hw, pl.hw, c.only_short};
+    ++*c.launches;
+    return launch_dependent(attention_quant_merge_kernel<HD>, dim3((unsigned)p.total_q * p.n_heads), dim3(MERGE_THREADS), 0, c.stream, c.pdl,
+                            p, (int)(c.dtype == DT_BF16), rows, c.grid / (p.n_kv / pl.hw), (const float *)c.ws);
 }
 
 bool mma_supported(const AttnQuant &p) { return (p.head_dim == 64 || p.head_dim == 128) && p.n_kv <= SHORT_MAX_GROUPS; }
@@ -1528,7 +1611,7 @@ cudaError_t launch_attention_quant(const AttnQuant &p, int dtype, float *ws, uin
     }
     const ShortPlan pl = short_plan(p, dtype);
     ShortCall c = {};
-    c.dtype = dtype; c.grid = short_grid(p, pl, sm_count); c.polls = polls; c.ws = ws; c.counters = counters; c.pdl = pdl; c.stream = s;
+    c.dtype = dtype; c.grid = short_grid(p, pl, sm_count); c.polls = polls; c.ws = ws; c.counters = counters; c.pdl = pdl; c.stream = s; c.launches = launches;
     c.tma = tma_fits(p);
     if (c.tma) {
         const cudaError_t e = encode_maps(p, pl.hw, &c.maps);

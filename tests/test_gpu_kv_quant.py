@@ -351,6 +351,7 @@ DECODE = [  # heads, kv heads, head_dim, page, lengths
     (32, 8, 128, 16, [1000]), (32, 8, 128, 16, [1]), (8, 8, 64, 32, [15, 16, 17]), (14, 2, 64, 24, [300, 1, 64, 63, 65]),
     (3, 1, 128, 1, [33, 2]), (40, 8, 128, 7, [129, 128, 127, 5]), (16, 1, 128, 64, [511]), (32, 1, 64, 16, [700, 3]),
     (17, 1, 128, 16, [90]), (4, 2, 256, 8, [300, 20]), (4, 4, 32, 16, [70]), (6, 2, 96, 5, [41, 200]), (5, 5, 160, 16, [77]),
+    (8, 4, 64, 16, [30000] + [20] * 9), (4, 2, 128, 16, [3 + 5 * i for i in range(70)]), (3, 1, 128, 32, [9000] * 2 + [1] * 8),
     (32, 8, 128, 256, [5000, 4097]), (7, 7, 128, 16, [260] * 9), (12, 3, 64, 48, [1025, 1024]), (32, 8, 128, 100000, [3000]),
 ]
 
@@ -365,6 +366,7 @@ SEVERAL = [  # heads, kv heads, head_dim, page, lengths, query tokens
     (32, 8, 128, 16, [200], [200]), (8, 2, 128, 16, [65], [64]), (8, 2, 64, 24, [300, 5, 77], [100, 1, 77]),
     (14, 2, 64, 16, [500, 40, 333], [129, 40, 1]), (4, 4, 128, 3, [150, 149], [127, 128]), (5, 1, 128, 16, [400], [33]),
     (16, 2, 128, 32, [130, 2, 600], [2, 2, 2]), (4, 1, 64, 16, [90, 91, 92], [4, 3, 5]), (32, 1, 128, 16, [260], [50]),
+    (8, 2, 128, 16, [200] * 3 + [90] * 9, [150, 1, 1] + [1] * 8 + [40]), (4, 1, 64, 24, [700] * 40, [1, 40] * 20),
     (6, 3, 96, 16, [70], [70]), (2, 2, 256, 16, [130], [40]), (32, 8, 128, 64, [1500], [600]), (8, 8, 128, 16, [1030], [1030]),
 ]
 

@@ -57,7 +57,7 @@ struct Request {
 };
 __device__ __forceinline__ Request request_of(const AttnQuant &p, int req) {
     const uint32_t a = min(p.query_starts[req], (uint32_t)p.total_q), b = min(p.query_starts[req + 1], (uint32_t)p.total_q);
-    const uint32_t room = (uint32_t)min((long long)p.max_blocks * p.block_size, 0x7FFFFFFFll);
+    const uint32_t room = (uint32_t)min((long long)p.max_blocks * p.block_size, 0x7FFF0000ll);      // positions, rounded up to tiles, stay ints
     uint32_t len = p.seq_lens[req];
     if (len > room) { report_error(p.err, KERR_SLOT_RANGE); len = room; }
     Request r;
@@ -998,7 +998,7 @@ __device__ __forceinline__ int f16_chunk_at(int row, int c) { return (c >> 3) * 
 
 template <int HD>
 __global__ void __launch_bounds__(LG_THREADS, 1)
-attention_quant_long_kernel(const AttnQuant p, int skip_short, uint32_t polls) {
+attention_quant_long_kernel(const AttnQuant p, int skip_short, int span, uint32_t polls) {
     using Sm = LongSmem<HD>;
     constexpr int CH = HD / 16;                          // 16-byte chunks of codes in a row
     extern __shared__ __align__(1024) uint8_t lg_smem[];
@@ -1023,7 +1023,7 @@ attention_quant_long_kernel(const AttnQuant p, int skip_short, uint32_t polls) {
         mbar_init_fence();
     }
     pdl_prologue();
-    // ---- which 256 rows: blocks of the requests in order, of a request the last (longest) ones first, KV heads innermost ----
+    // ---- which rows (span: 256, or 128 for tile 0 alone): blocks of the requests in order, of a request the last (longest) ones first, KV heads innermost ----
     const int group = p.n_heads / p.n_kv, kvh = blockIdx.x % p.n_kv;
     int want = blockIdx.x / p.n_kv, req = -1;
     Request r = {0, 0, 0};
@@ -1033,7 +1033,7 @@ attention_quant_long_kernel(const AttnQuant p, int skip_short, uint32_t polls) {
         if (q0 + lane < p.num_req) {
             mine = request_of(p, q0 + lane);
             const long long rows = (long long)mine.count * group;
-            blocks = skip_short && rows <= SHORT_ROWS ? 0 : (int)((rows + 2 * LG_ROWS - 1) / (2 * LG_ROWS));
+            blocks = skip_short && rows <= SHORT_ROWS ? 0 : (int)((rows + span - 1) / span);
         }
         int inc = blocks;
 #pragma unroll
@@ -1054,7 +1054,7 @@ attention_quant_long_kernel(const AttnQuant p, int skip_short, uint32_t polls) {
         }
     }
     if (req < 0) return;                                 // the grid holds as many CTAs as any batch of this size can need
-    const int row0 = want * 2 * LG_ROWS, rows = r.count * group - row0;          // of this CTA: 1 .. 256 are used
+    const int row0 = want * span, rows = min(r.count * group - row0, span);      // of this CTA: 1 .. 256
     // positions that tile t's last row sees, and tiles of positions
     int nt[2];
 #pragma unroll
@@ -1064,7 +1064,7 @@ attention_quant_long_kernel(const AttnQuant p, int skip_short, uint32_t polls) {
         nt[t] = end > 0 ? (end + LG_POS - 1) / LG_POS : 0;
     }
     const int n_tiles = max(nt[0], nt[1]);               // tile 1's rows come later and see more, if there are any
-    const int kv_end = r.before + (row0 + min(rows, 2 * LG_ROWS) - 1) / group + 1;
+    const int kv_end = r.before + (row0 + rows - 1) / group + 1;
     if (warp == 16) { tmem_alloc(&tmem_base_s, 512); tmem_relinquish(); }
     tc_fence_before();
     __syncthreads();
@@ -1418,14 +1418,20 @@ attention_quant_long_kernel(const AttnQuant p, int skip_short, uint32_t polls) {
 }
 
 template <int HD>
-cudaError_t launch_long(const AttnQuant &p, int skip_short, uint32_t polls, cudaStream_t s, bool pdl) {
-    const int group = p.n_heads / p.n_kv;
-    const long long blocks = ((long long)p.total_q * group + 2 * LG_ROWS - 1) / (2 * LG_ROWS) + p.num_req;
+cudaError_t launch_long(const AttnQuant &p, int skip_short, int sm_count, uint32_t polls, cudaStream_t s, bool pdl) {
+    // 256 rows a CTA, so that two tiles share keys and values and hide each other's waits; one tile of 128 where that is about
+    // a CTA an SM or less (1.25: requests differ in length).  128 tokens of 32 heads over 8: 11.9 us with one tile, 16.4 with
+    // two; 128 behind 8064: 140 and 160; 12 chunks of up to 500 tokens, 2 KV heads: 76 and 88; but 1152 tokens: 40.5 and 36.6.
+    const long long rows = (long long)p.total_q * (p.n_heads / p.n_kv);
+    const int span = rows * p.n_kv <= (long long)sm_count * LG_ROWS * 5 / 4 ? LG_ROWS : 2 * LG_ROWS;
+    // every request may end in a block that is not full; the short kernel's, of at most SHORT_ROWS rows, have none
+    const long long ends = skip_short && rows / (SHORT_ROWS + 1) < p.num_req ? rows / (SHORT_ROWS + 1) : p.num_req;
+    const long long blocks = (rows + span - 1) / span + ends;
     const cudaError_t e = cudaFuncSetAttribute(attention_quant_long_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, LongSmem<HD>::BYTES);
     if (e != cudaSuccess) return e;
     if (blocks * p.n_kv > 0x7FFFFFFFll) return cudaErrorInvalidValue;
     return launch_dependent(attention_quant_long_kernel<HD>, dim3((unsigned)(blocks * p.n_kv)), dim3(LG_THREADS), LongSmem<HD>::BYTES, s, pdl, p,
-                            skip_short, polls);
+                            skip_short, span, polls);
 }
 
 struct ShortPlan { int rb, terms, hw, per_sm; };
@@ -1624,7 +1630,7 @@ cudaError_t launch_attention_quant(const AttnQuant &p, int dtype, float *ws, uin
     const bool decode = p.total_q <= p.num_req || rows <= SHORT_ROWS;
     if (dtype == DT_BF16 && !decode) {
         const int both = p.num_req > 1;
-        cudaError_t e = p.head_dim == 128 ? launch_long<128>(p, both, polls, s, pdl) : launch_long<64>(p, both, polls, s, pdl);
+        cudaError_t e = p.head_dim == 128 ? launch_long<128>(p, both, sm_count, polls, s, pdl) : launch_long<64>(p, both, sm_count, polls, s, pdl);
         ++*launches;
         if (e != cudaSuccess || !both) return e;
         c.only_short = 1;

@@ -79,7 +79,7 @@ template <int V> __device__ __forceinline__ void codes_of(uint32_t (&w)[V < 4 ? 
 // E4M3(x / scale) of V finite values, as IEEE division would have it, mostly without dividing: x times 1 / scale is off by
 // less than 2^-22 of itself (two roundings), so the quotient lies between the products with inv (1 - 2^-22) and
 // inv (1 + 2^-22); where both round to one code that is the quotient's.  A quotient near the middle between two
-// codes, a few of a million, is divided.  (Dividing everything: 53 us instead of 33 for 8192 tokens.)
+// codes, a few of a million, is divided.  (8192 tokens rotated and written: 49.5 us, dividing everything 52.9.)
 template <int V> __device__ __forceinline__ void store_codes(uint8_t *p, const float *x, float scale, float inv) {
     constexpr int W = V < 4 ? 1 : V / 4;
     uint32_t w[W], v[W];
@@ -113,7 +113,9 @@ __device__ __forceinline__ void rotate(float &a, float &b, float2 t) {
 // The cosines and sines of a token are formed once per CTA (one per thread, angle reduced in float64: at
 // position 131072 a float32 angle has lost 7 of its fraction's bits) and shared by its 40 or so heads.
 // HBM-bound: what is read and written is what the operation cannot do without.  So a thread asks for the units of
-// PRE rows before anything else; the angles are formed while they are under way.
+// PRE rows before anything else; the angles are formed while they are under way.  8192 tokens, 32 + 8 heads of 128, bf16:
+// rotated 30.9 us (5.4 TB/s, 83 % of the measured rate); rotated and written 43.4 (65 %), there bound by issue slots, the
+// rows that are quantised taking twice the instructions of the others.
 template <typename T, int V, int ITER, int PRE, bool HALF>
 __global__ void __launch_bounds__(RW_THREADS, ITER == 1 ? 7 : 1) rope_write_kernel(const RopeWrite p) {
     using C = Chunk<T, V>;
@@ -228,7 +230,8 @@ __global__ void __launch_bounds__(RW_THREADS, ITER == 1 ? 7 : 1) rope_write_kern
 }
 
 // Rows read back: out[c] = codes of slot indices[c], each head's times its scale; one product and one rounding.  A thread
-// takes V codes of one head at a time (32 bytes of output, one store), of N units at once.  HBM-bound.
+// takes V codes of one head at a time (32 bytes of output, one store), of N units at once.  HBM-bound: 40001 rows of 1024
+// to float32 34.6 us (6.0 TB/s, 91 % of the measured rate; 59.8 with 4 codes a thread).
 template <typename T, int V> __device__ __forceinline__ void store_row(T *p, const float *x) {
     if constexpr (V == 1) {
         Chunk<T, 1>::store(p, x);

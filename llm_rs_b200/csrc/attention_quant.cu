@@ -153,7 +153,7 @@ __global__ void __launch_bounds__(AQ_TILE) attention_quant_simple_kernel(const A
 // HBM-bound: a position's 2 head_dim codes and two scales are read once for all the query rows of its KV head.
 //
 // Work.  A row block is up to RB rows (query token x head of the group) of one request and KV head; a unit is a
-// row block's next 16 PW positions, PW = 8 / HW, for HW KV heads at once.  The units of all requests form one
+// row block's next 32 PW positions, PW = 4 / HW, for HW KV heads at once.  The units of all requests form one
 // sequence that is cut into equal contiguous ranges, one per CTA, so ragged batches load every SM alike and one
 // long request spreads over the whole GPU.  The lengths are on the device, so each CTA adds them up itself.  A row
 // block that lies in several ranges leaves (accumulator, maximum, sum) parts in the workspace; the last CTA to finish of
@@ -163,8 +163,9 @@ __global__ void __launch_bounds__(AQ_TILE) attention_quant_simple_kernel(const A
 // One request of 131071 positions: 57 us, 74 % of the measured HBM rate; without the joining 49 (86 %).  64 requests of
 // 100 to 8192: 108 us, 79 %; without 97 (88 %).
 //
-// A CTA has 8 consumer warps, HW heads x PW runs of 16 positions, so that neighbouring heads of a slot, neighbours
-// in memory, are read at the same time, and a producer that keeps NST units in flight, through to the end of the
+// A CTA has 4 consumer warps, HW heads x PW times 32 positions, so that neighbouring heads of a slot, neighbours
+// in memory, are read at the same time (one head a CTA: 142 us for the 64 requests; 16 positions a warp instead of 32: 69 us
+// instead of 60 for the one, at that step), and a producer that keeps NST units in flight, through to the end of the
 // CTA's range.  Where 16 positions never straddle a page (block_size a multiple of 16, and the scales' rows 16-byte
 // aligned) the producer is one thread that issues four tiled TMA copies per 16 positions of all the heads; otherwise
 // four warps fetch 16 bytes a lane.  (The first form had every warp fetch for itself: 692 instructions a warp per 16
@@ -1458,6 +1459,8 @@ size_t short_workspace(const AttnQuant &p, const ShortPlan &s, int sm_count) {
 }
 
 constexpr int MERGE_THREADS = 512, MERGE_REQUESTS = 8;       // of attention_quant_merge_kernel
+// Few requests, and few rows, since it starts a CTA for each row of the batch, whether or not that was split.
+bool merges_after(const AttnQuant &p) { return p.num_req <= MERGE_REQUESTS && p.total_q <= SHORT_ROWS * MERGE_REQUESTS; }
 // What the launches of one call share.
 struct ShortCall {
     ShortMaps maps;
@@ -1501,7 +1504,7 @@ cudaError_t launch_short(const AttnQuant &p, const ShortCall &c) {
     const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;
     return launch_dependent(k, dim3((unsigned)c.grid), dim3(SH_THREADS + (TMA ? 32 : 128)), smem, c.stream, c.pdl, c.maps, p,
-                            (int)(c.dtype == DT_BF16), c.only_short, c.polls, c.ws, c.counters, (int)(p.num_req > MERGE_REQUESTS));
+                            (int)(c.dtype == DT_BF16), c.only_short, c.polls, c.ws, c.counters, (int)!merges_after(p));
 }
 template <int HD, int RB, int TERMS, int NST>
 cudaError_t launch_short_hw(const AttnQuant &p, int hw, const ShortCall &c) {
@@ -1589,7 +1592,7 @@ cudaError_t launch_short_all(const AttnQuant &p, const ShortPlan &pl, const Shor
     cudaError_t e;
     if (pl.terms == 2) e = pl.rb == 8 ? launch_short_hw<HD, 8, 2, NST>(p, pl.hw, c) : launch_short_hw<HD, 16, 2, NST>(p, pl.hw, c);
     else e = pl.rb == 8 ? launch_short_hw<HD, 8, 1, NST>(p, pl.hw, c) : launch_short_hw<HD, 16, 1, NST>(p, pl.hw, c);
-    if (e != cudaSuccess || p.num_req > MERGE_REQUESTS) return e;
+    if (e != cudaSuccess || !merges_after(p)) return e;
     const Rows rows{pl.rb, 16 * SH_TILES / pl.hw, pl.hw, c.only_short};
     ++*c.launches;
     return launch_dependent(attention_quant_merge_kernel<HD>, dim3((unsigned)p.total_q * p.n_heads), dim3(MERGE_THREADS), 0, c.stream, c.pdl,

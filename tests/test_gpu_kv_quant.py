@@ -367,6 +367,7 @@ SEVERAL = [  # heads, kv heads, head_dim, page, lengths, query tokens
     (14, 2, 64, 16, [500, 40, 333], [129, 40, 1]), (4, 4, 128, 3, [150, 149], [127, 128]), (5, 1, 128, 16, [400], [33]),
     (16, 2, 128, 32, [130, 2, 600], [2, 2, 2]), (4, 1, 64, 16, [90, 91, 92], [4, 3, 5]), (32, 1, 128, 16, [260], [50]),
     (8, 2, 128, 16, [200] * 3 + [90] * 9, [150, 1, 1] + [1] * 8 + [40]), (4, 1, 64, 24, [700] * 40, [1, 40] * 20),
+    (8, 2, 128, 16, [100] + [5] * 50, [40] + [0] * 50), (8, 1, 64, 16, [300] * 3, [17, 1, 2]),
     (6, 3, 96, 16, [70], [70]), (2, 2, 256, 16, [130], [40]), (32, 8, 128, 64, [1500], [600]), (8, 8, 128, 16, [1030], [1030]),
 ]
 
@@ -484,6 +485,27 @@ def test_attention_lengths_and_starts_beyond_what_there_is(backend):
     backend.sync()
     want, slack = expected(q, kc, ks, vc, vs, slots, [48], [2], nh, nkv, hd)
     assert ((out.double() - want).abs() <= 2.0 ** -8 * 1.01 * want.abs() + slack).all()
+
+
+def test_attention_needs_its_workspace_before_a_capture(cuda_lib):
+    """A first call inside a capture would have to allocate: refused, and the context goes on."""
+    stream = torch.cuda.Stream()
+    be = CudaBackend(0, stream.cuda_stream)
+    kc, ks, vc, vs, table, slots, most = paged_cache(2, 64, [40], 16, 85)
+    q, out = torch.zeros(1, 256, dtype=torch.bfloat16, device="cuda"), torch.zeros(1, 256, dtype=torch.bfloat16, device="cuda")
+    b = [buf(be, t) for t in (out, q, kc, ks, vc, vs, table, ints([0, 1]), ints([40]))]
+    torch.cuda.synchronize()
+    graph, refused = torch.cuda.CUDAGraph(), None
+    with torch.cuda.graph(graph, stream=stream):
+        try:
+            be.attention_quant(*b, 4, 2, 64, 16, most)
+        except BackendError as e:
+            refused = e
+    assert refused is not None and refused.code == -1 and "capture" in str(refused)
+    be.attention_quant(*b, 4, 2, 64, 16, most)
+    be.sync()
+    assert out.isfinite().all() and out.any()            # queries of zeros: the mean of the values
+    be.close()
 
 
 def test_attention_twice_is_the_same(backend):

@@ -270,40 +270,48 @@ def run(state):
 
 # ---- the framework's calls -----------------------------------------------------------------------
 
-_backend = None
+_backends = {}
+LEGACY_STREAM = 1          # the handle that names torch's default stream; 0 asks for a stream of the context's own
 
 
-def _buffers(state):
+def _backend():
+    """A context on torch's current stream: its calls come after what torch has put there and before what it puts there next."""
+    from llm_rs_b200 import CudaBackend
+    at = torch.cuda.current_device(), torch.cuda.current_stream().cuda_stream or LEGACY_STREAM
+    if at not in _backends:
+        _backends[at] = CudaBackend(*at)
+    return _backends[at]
+
+
+def _buffers(backend, state):
     """The state's tensors as buffers of the framework, which a program that keeps its data there has from the start."""
-    global _backend
-    from llm_rs_b200 import CudaBackend, DType
-    if _backend is None:
-        _backend = CudaBackend(torch.cuda.current_device())
+    from llm_rs_b200 import DType
     kinds = {torch.bfloat16: DType.BF16, torch.float32: DType.F32, torch.int32: DType.I32, torch.float8_e4m3fn: DType.E4M3}
-    return {n: _backend.wrap(t.data_ptr(), t.shape[::-1], kinds[t.dtype], keepalive=t)
+    return {n: backend.wrap(t.data_ptr(), t.shape[::-1], kinds[t.dtype], keepalive=t)
             for n, t in state.items() if isinstance(t, torch.Tensor)}
 
 
 def _run_own(state):
     s, case = state, state["case"]
-    b = s.get("buffers")
-    if b is None:
-        b = s["buffers"] = _buffers(s)
+    if "buffers" not in s:                              # the context and the buffers, as a program keeps them
+        s["backend"] = _backend()
+        s["buffers"] = _buffers(s["backend"], s)
+    be, b = s["backend"], s["buffers"]
     if case["op"] == "attention":
-        _backend.attention_quant(b["out"], b["q"], b["k_codes"], b["k_scales"], b["v_codes"], b["v_scales"], b["table"],
-                                 b["starts"], b["lens"], case["heads"], case["kv_heads"], case["head_dim"], case["page"],
-                                 s["table"].shape[1])
+        be.attention_quant(b["out"], b["q"], b["k_codes"], b["k_scales"], b["v_codes"], b["v_scales"], b["table"],
+                           b["starts"], b["lens"], case["heads"], case["kv_heads"], case["head_dim"], case["page"],
+                           s["table"].shape[1])
         return s["out"]
     if case["op"] == "read":
-        _backend.gather_quant(b["out"], b["codes"], b["scales"], b["rows"], case["rows"])
+        be.gather_quant(b["out"], b["codes"], b["scales"], b["rows"], case["rows"])
         return s["out"]
     if case["op"] == "rope":
-        _backend.rope_scaled(b["q_out"], b["k_out"], b["q"], b["k"], b["positions"], b["freq"], case["head_dim"],
-                             s["magnitude"], split_half=case["half"])
+        be.rope_scaled(b["q_out"], b["k_out"], b["q"], b["k"], b["positions"], b["freq"], case["head_dim"],
+                       s["magnitude"], split_half=case["half"])
         return [s["q_out"], s["k_out"]]
-    _backend.rope_scatter_kv_quant(b["q_out"], b["q"], b["k"], b["v"], b["positions"], b["freq"], case["head_dim"],
-                                   s["magnitude"], b["k_codes"], b["k_scales"], b["v_codes"], b["v_scales"], b["slots"],
-                                   split_half=case["half"])
+    be.rope_scatter_kv_quant(b["q_out"], b["q"], b["k"], b["v"], b["positions"], b["freq"], case["head_dim"],
+                             s["magnitude"], b["k_codes"], b["k_scales"], b["v_codes"], b["v_scales"], b["slots"],
+                             split_half=case["half"])
     return [s["q_out"], s["k_codes"], s["k_scales"], s["v_codes"], s["v_scales"]]
 
 

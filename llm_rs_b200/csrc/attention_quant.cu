@@ -911,7 +911,7 @@ attention_quant_short_kernel(const __grid_constant__ ShortMaps maps, const AttnQ
 //   warps 0-3, 4-7   weights of tile 0, 1: a thread owns a row.  Scores come from TMEM 16 columns at a time, weights go back
 //                    as f16 over the scores that they came from.
 //   warps 8-11, 12-15   keys, values: codes to shared memory as they are, one tile ahead, then to f16 in the 128-byte
-//                    swizzle, the scales multiplied in.  Any page size: rows are looked up one by one.
+//                    swizzle; the scales beside them.  Any page size: rows are looked up one by one.
 //   warp 16          issues the products: S = Q K^T (both from shared memory), O += W V (W from TMEM; the values lie
 //                    as they come, positions in rows, so they are the operand's major dimension the other way round).
 //
@@ -919,25 +919,24 @@ attention_quant_short_kernel(const __grid_constant__ ShortMaps maps, const AttnQ
 // is rarely rescaled (2 instead of 6: 4096 tokens 207 us instead of 191); weights then stay below 64, and enter as
 // e^(s - m) * 2^9: f16 keeps 2^-11 of a weight, and down to 2^-34 of the largest.
 //
-// The scales are multiplied into the f16 keys and values as these are made, once a code instead of once a score (scales
-// at the scores: 227 us): a key is code * ks / (least power of two that no ks of its tile exceeds) * 2^6, a value code * vs / R
-// * 2^6 (R as in the other kernel).  The product is rounded to f16, 2^-11 of itself at most; a key's ks enters as two f16, so
-// that nothing common to a whole score is rounded; a value's as one, 2^-11 more of a weight.  Scales below 2^-20 of
-// the power lose further bits: a value is kept to 2^-30 of the largest before it.  A value whose scale is not finite is
-// zero there, and the rows that see it are marked, so that no row sees NaN times zero.
-//
-// 128 query rows a tile, 4096 tokens of 32 heads over 8: 0.7 PFLOP/s; 1152 tokens behind 31616: 1.0 (59 % of measured).  What
-// is left there is the issue of the weights' 3.5 instructions a score and, for short prompts, a CTA's start and end
-// (about 8 us: lookups, queries, first keys; one CTA fits an SM).
+// The codes, exact in f16, are what is multiplied; ks enters at the score and vs / R at the weight, in float32 (R as in the other
+// kernel).  Multiplied into the f16 keys and values instead, once a code and not once a score, they make the weights 1.75
+// instructions a score shorter (4096 tokens 200 us instead of 242), but every product is then rounded to 2^-11: a weight
+// behind a score of 300 is off by a tenth.  A value whose scale is not finite is zero there, and the rows that see it are marked,
+// so that no row sees NaN times zero.
 constexpr int LG_ROWS = 128, LG_POS = 128, LG_THREADS = 17 * 32;
 constexpr float LG_SLACK = 6.0f;     // log2: the weights' factor 2^9 leaves these octaves to f16's 65504
 
+struct LongFlags {                   // of a tile of positions, 32 to a warp
+    uint32_t there[4];               // which of them are
+    uint32_t bad[4];                 // whose value's scale is not finite
+    uint32_t big[4];                 // whose key's scale is above 2^90
+    uint32_t all, r_bits;            // nothing of this needs a look; R
+};
 template <int HD> struct LongSmem {
     static constexpr int HALVES = HD / 64, TILE = LG_ROWS * HD * 2;      // 128 rows of f16, in halves of 64 dimensions
     static constexpr int Q = 0, K = 2 * TILE, V = K + 2 * TILE, RAW = V + 2 * TILE, SC = RAW + 2 * (TILE / 2);
-    // of a tile of positions: which are there [4], whose value's scale is not finite [4], whether nothing of this needs a
-    // look, R's bits, the factor of its scores
-    static constexpr int STAGES = 3, MASK = 0, BAD = 16, ALL = 32, RBITS = 36, KREF = 40, SCALES = 64;
+    static constexpr int STAGES = 2, KS = 0, VW = 512, SCALES = 1024;    // of a tile of positions: ks [128], vs / R [128]
     static constexpr int BYTES = SC + STAGES * SCALES;
 };
 
@@ -1004,7 +1003,8 @@ attention_quant_long_kernel(const AttnQuant p, int skip_short, int span, uint32_
     constexpr int CH = HD / 16;                          // 16-byte chunks of codes in a row
     extern __shared__ __align__(1024) uint8_t lg_smem[];
     __shared__ __align__(8) uint64_t q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], sc_full[Sm::STAGES], sc_empty[Sm::STAGES], s_full[2], p_full[2], o_full[2];
-    __shared__ uint32_t tmem_base_s, top_s[2][2][4], look_s[2][4];
+    __shared__ LongFlags flags_s[Sm::STAGES];
+    __shared__ uint32_t tmem_base_s, top_s[2][4], look_s[2][4];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if (tid == 0) {
         for (int i = 0; i < 2; i++) {
@@ -1118,14 +1118,15 @@ attention_quant_long_kernel(const AttnQuant p, int skip_short, int span, uint32_
             wait(&sc_full[st], (j / Sm::STAGES) & 1, KERR_FULL_WAIT);
             if (j < nt[t]) {
                 const uint8_t *sc = lg_smem + Sm::SC + st * Sm::SCALES;
-                const float c_tile = c_row * *reinterpret_cast<const float *>(sc + Sm::KREF);
-                const uint32_t r_new = *reinterpret_cast<const uint32_t *>(sc + Sm::RBITS);
-                const bool masked = !full_tile || (j + 1) * LG_POS > min_len || *reinterpret_cast<const uint32_t *>(sc + Sm::ALL) == 0;
+                const float *ks = reinterpret_cast<const float *>(sc + Sm::KS), *vw = reinterpret_cast<const float *>(sc + Sm::VW);
+                const LongFlags &fl = flags_s[st];
+                const uint32_t r_new = fl.r_bits;
+                const bool masked = !full_tile || (j + 1) * LG_POS > min_len || fl.all == 0 || (fl.big[0] | fl.big[1] | fl.big[2] | fl.big[3]) != 0;
                 wait(&s_full[t], j & 1, KERR_MMA_WAIT);
                 tc_fence_after();
                 auto bits_of = [&](int c) -> uint32_t {  // which of the 32 positions of chunk c this row sees
                     const int n = len - j * LG_POS - 32 * c;
-                    const uint32_t there = *reinterpret_cast<const uint32_t *>(sc + Sm::MASK + 4 * c);
+                    const uint32_t there = fl.there[c];
                     return n <= 0 ? 0u : n >= 32 ? there : there & ((1u << n) - 1);
                 };
                 // Two forms of the code, chosen by the warp: most tiles are seen by every row whole, and a test a score costs
@@ -1133,6 +1134,13 @@ attention_quant_long_kernel(const AttnQuant p, int skip_short, int span, uint32_
                 auto work = [&](auto mask_tag) {
                     constexpr bool MASKED = decltype(mask_tag)::value;
                     uint32_t v[2][16];
+                    // A sum of codes and queries is below 2^30; times a scale of 2^98 it would leave float32 before the row's
+                    // factor brings it back, so the masked form multiplies scale and factor first.
+                    const float2 c2 = make_float2(c_row, c_row);
+                    auto scaled = [&](float a, float b, float ka, float kb) {
+                        const float2 k2 = MASKED ? pair_mul(make_float2(ka, kb), c2) : make_float2(ka, kb);
+                        return pair_mul(make_float2(a, b), k2);
+                    };
                     // ---- the row's maximum ----
                     float mx0 = -INFINITY, mx1 = -INFINITY;
                     tmem_ld16(s_col, v[0]);
@@ -1145,19 +1153,21 @@ attention_quant_long_kernel(const AttnQuant p, int skip_short, int span, uint32_
                         if constexpr (MASKED) bits = bits_of(c >> 1) >> (16 * (c & 1));
 #pragma unroll
                         for (int x = 0; x < 16; x += 4) {
-                            float a[4];
-#pragma unroll
-                            for (int y = 0; y < 4; y++) {
-                                a[y] = __uint_as_float(u[x + y]);
-                                if constexpr (MASKED)
-                                    if (!(bits >> (x + y) & 1)) a[y] = -INFINITY;
+                            const float4 k4 = *reinterpret_cast<const float4 *>(ks + 16 * c + x);
+                            float2 a = scaled(__uint_as_float(u[x]), __uint_as_float(u[x + 1]), k4.x, k4.y);
+                            float2 d = scaled(__uint_as_float(u[x + 2]), __uint_as_float(u[x + 3]), k4.z, k4.w);
+                            if constexpr (MASKED) {
+                                if (!(bits >> x & 1)) a.x = -INFINITY;
+                                if (!(bits >> (x + 1) & 1)) a.y = -INFINITY;
+                                if (!(bits >> (x + 2) & 1)) d.x = -INFINITY;
+                                if (!(bits >> (x + 3) & 1)) d.y = -INFINITY;
                             }
-                            mx0 = fmaxf(mx0, fmaxf(a[0], a[1]));
-                            mx1 = fmaxf(mx1, fmaxf(a[2], a[3]));
+                            mx0 = fmaxf(mx0, fmaxf(a.x, a.y));
+                            mx1 = fmaxf(mx1, fmaxf(d.x, d.y));
                         }
                         tmem_ld_wait();
                     }
-                    const float mx = fmaxf(mx0, mx1) * c_tile;
+                    const float mx = MASKED ? fmaxf(mx0, mx1) : fmaxf(mx0, mx1) * c_row;
                     // ---- move the reference, O and the sum where the maximum has outgrown it ----
                     const float m_new = mx > m_ref + LG_SLACK ? mx : m_ref;      // m_ref = -inf: any score at all
                     const bool moved = m_new != m_ref || r_new != r_bits;
@@ -1180,9 +1190,8 @@ attention_quant_long_kernel(const AttnQuant p, int skip_short, int span, uint32_
                     m_ref = m_new;
                     r_bits = r_new;
                     // ---- the weights, over the scores ----
-                    const float2 c2 = make_float2(c_tile, c_tile), nb = make_float2(9.0f - base, 9.0f - base);
+                    const float2 nb = make_float2(9.0f - base, 9.0f - base), one2 = make_float2(1.0f, 1.0f);
                     bool bad = false;
-#pragma unroll
                     uint32_t w[16];
 #pragma unroll
                     for (int c = 0; c < 8; c++) {
@@ -1191,20 +1200,27 @@ attention_quant_long_kernel(const AttnQuant p, int skip_short, int span, uint32_
                         uint32_t bits = 0;
                         if constexpr (MASKED) {
                             bits = bits_of(c >> 1);
-                            bad = bad || (bits & *reinterpret_cast<const uint32_t *>(sc + Sm::BAD + 4 * (c >> 1))) != 0;
+                            bad = bad || (bits & fl.bad[c >> 1]) != 0;
                             bits >>= 16 * (c & 1);
                         }
 #pragma unroll
-                        for (int x = 0; x < 16; x += 2) {
-                            float2 e = pair_op(make_float2(__uint_as_float(u[x]), __uint_as_float(u[x + 1])), c2, nb);
-                            e.x = ex2(e.x);
-                            e.y = ex2(e.y);
-                            if constexpr (MASKED) {
-                                if (!(bits >> x & 1)) e.x = 0.0f;
-                                if (!(bits >> (x + 1) & 1)) e.y = 0.0f;
+                        for (int x = 0; x < 16; x += 4) {
+                            const float4 k4 = *reinterpret_cast<const float4 *>(ks + 16 * c + x), w4 = *reinterpret_cast<const float4 *>(vw + 16 * c + x);
+#pragma unroll
+                            for (int y = 0; y < 2; y++) {
+                                const int at = x + 2 * y;
+                                float2 e = scaled(__uint_as_float(u[at]), __uint_as_float(u[at + 1]), y ? k4.z : k4.x, y ? k4.w : k4.y);
+                                e = MASKED ? pair_op(e, one2, nb) : pair_op(e, c2, nb);
+                                e.x = ex2(e.x);
+                                e.y = ex2(e.y);
+                                if constexpr (MASKED) {
+                                    if (!(bits >> at & 1)) e.x = 0.0f;
+                                    if (!(bits >> (at + 1) & 1)) e.y = 0.0f;
+                                }
+                                l2 = pair_add(l2, e);
+                                e = pair_mul(e, y ? make_float2(w4.z, w4.w) : make_float2(w4.x, w4.y));
+                                w[8 * (c & 1) + at / 2] = pack_f16(e.x, e.y);
                             }
-                            l2 = pair_add(l2, e);
-                            w[8 * (c & 1) + x / 2] = pack_f16(e.x, e.y);
                         }
                         if (c < 7) tmem_ld_wait();
                         if (c & 1) tmem_st16(s_col + 16 * (c >> 1), w);
@@ -1222,7 +1238,7 @@ attention_quant_long_kernel(const AttnQuant p, int skip_short, int span, uint32_
         }
         // ---- O, divided by the sum ----
         const float l = l2.x + l2.y;
-        const float norm = l == 0.0f ? 0.0f : __uint_as_float(r_bits - (6u << 23)) / l;
+        const float norm = l == 0.0f ? 0.0f : __uint_as_float(r_bits) / l;
         uint16_t *out = (uint16_t *)p.out + off;
         if (nt[t] > 0) {
             wait(&o_full[t], 0, KERR_MMA_WAIT);
@@ -1287,8 +1303,7 @@ attention_quant_long_kernel(const AttnQuant p, int skip_short, int span, uint32_
             asm volatile("cp.async.commit_group;" ::: "memory");
             page = page_of(j + 1);
         };
-        auto power_above = [](uint32_t bits) { return min((bits + 0x7FFFFFu) & 0x7F800000u, 253u << 23); };      // of two
-        uint32_t power = 17u << 23;                      // values: R, which only grows; keys: of the tile
+        uint32_t power = 17u << 23;                      // R, which only grows
         if (n_tiles > 0) {
             page = page_of(0);
             ask(0);
@@ -1298,63 +1313,59 @@ attention_quant_long_kernel(const AttnQuant p, int skip_short, int span, uint32_
             const uint32_t there = there_next;
             const bool ok = keys || scale_next <= 3.402823466e38f;       // a value's scale that is NaN or infinite: zeros, and marked
             const float scale = ok ? scale_next : 0.0f;
-            float top = fmaxf(0.0f, scale);
+            auto publish = [&]() {
+                uint8_t *sc = lg_smem + Sm::SC + st * Sm::SCALES;
+                LongFlags &fl = flags_s[st];
+                if (keys) {
+                    const uint32_t big = __ballot_sync(0xffffffffu, fabsf(scale) > 0x1p90f);
+                    if (j >= Sm::STAGES) wait(&sc_empty[st], ((j / Sm::STAGES) & 1) ^ 1, KERR_EMPTY_WAIT);
+                    reinterpret_cast<float *>(sc + Sm::KS)[32 * w + lane] = scale;
+                    if (lane == 0) {
+                        fl.there[w] = there;
+                        fl.big[w] = big;
+                    }
+                } else {
+                    float top = fmaxf(0.0f, scale);
 #pragma unroll
-            for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-            const uint32_t bad = __ballot_sync(0xffffffffu, !ok);
-            if (lane == 0) {
-                top_s[keys][b][w] = __float_as_uint(top);
-                if (!keys) look_s[b][w] = there != 0xFFFFFFFFu || bad;   // positions past kv_end, on a page beyond the pool, or marked
-            }
-            named_barrier_sync(keys ? 2 : 3, 128);       // what the four warps have found
-            const uint32_t *tops = top_s[keys][b];
-            const uint32_t above = power_above(max(max(tops[0], tops[1]), max(tops[2], tops[3])));
-            power = max(keys ? 17u << 23 : power, above);
-            if (j >= Sm::STAGES) wait(&sc_empty[st], ((j / Sm::STAGES) & 1) ^ 1, KERR_EMPTY_WAIT);
-            uint8_t *sc = lg_smem + Sm::SC + st * Sm::SCALES;
-            if (keys) {
-                if (lane == 0) reinterpret_cast<uint32_t *>(sc + Sm::MASK)[w] = there;
-                if (w == 0 && lane == 0) *reinterpret_cast<uint32_t *>(sc + Sm::KREF) = power - (6u << 23);
-            } else {
-                if (lane == 0) reinterpret_cast<uint32_t *>(sc + Sm::BAD)[w] = bad;
-                if (w == 0 && lane == 0) {
-                    *reinterpret_cast<uint32_t *>(sc + Sm::ALL) = !(look_s[b][0] | look_s[b][1] | look_s[b][2] | look_s[b][3]);
-                    *reinterpret_cast<uint32_t *>(sc + Sm::RBITS) = power;
+                    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                    const uint32_t bad = __ballot_sync(0xffffffffu, !ok);
+                    if (lane == 0) {
+                        top_s[b][w] = __float_as_uint(top);
+                        look_s[b][w] = there != 0xFFFFFFFFu || bad;      // positions past kv_end, on a page beyond the pool, or marked
+                    }
+                    named_barrier_sync(2, 128);          // what the four warps have found
+                    const uint32_t most = max(max(top_s[b][0], top_s[b][1]), max(top_s[b][2], top_s[b][3]));
+                    power = max(power, min((most + 0x7FFFFFu) & 0x7F800000u, 253u << 23));
+                    if (j >= Sm::STAGES) wait(&sc_empty[st], ((j / Sm::STAGES) & 1) ^ 1, KERR_EMPTY_WAIT);
+                    reinterpret_cast<float *>(sc + Sm::VW)[32 * w + lane] = scale * __uint_as_float((254u << 23) - power);
+                    if (lane == 0) fl.bad[w] = bad;
+                    if (w == 0 && lane == 0) {
+                        fl.all = !(look_s[b][0] | look_s[b][1] | look_s[b][2] | look_s[b][3]);
+                        fl.r_bits = power;
+                    }
                 }
-            }
-            mbar_arrive(&sc_full[st]);
-            // The scale over the power of two, times 2^6, as f16 hi + lo; a value does with hi, whose 2^-12 is one more rounding
-            // of a weight, a key's score would be off by as much of itself.
-            const float fs = scale * __uint_as_float(((127u + 127u + 6u) << 23) - power);
-            const __half hi = __float2half_rn(fs), lo = __float2half_rn(keys ? fs - __half2float(hi) : 0.0f);
-            const uint32_t pair = (uint32_t)__half_as_ushort(hi) | (uint32_t)__half_as_ushort(lo) << 16;
+                mbar_arrive(&sc_full[st]);
+            };
+            if (!keys) publish();                        // the weights wait for the scales, the keys' product for the keys
             if (j >= 2) wait(&empty[b], ((j >> 1) & 1) ^ 1, KERR_EMPTY_WAIT);
             asm volatile("cp.async.wait_group 0;" ::: "memory");
             uint8_t *tile = tiles + b * Sm::TILE;
-            auto convert = [&](auto key_tag) {
 #pragma unroll
-                for (int x = 0; x < N; x++) {
-                    const int row = x * RPI + lane / CH;
-                    const uint32_t f = __shfl_sync(0xffffffffu, pair, row), f_hi = h2_bcast_lo(f), f_lo = h2_bcast_hi(f);
-                    const uint4 u = *reinterpret_cast<const uint4 *>(raw + row * HD + 16 * c);
-                    const uint32_t r4[4] = {u.x, u.y, u.z, u.w};
-                    uint32_t h[8];
-#pragma unroll
-                    for (int y = 0; y < 4; y++) codes_to_f16(r4[y], h[2 * y], h[2 * y + 1]);
-#pragma unroll
-                    for (int y = 0; y < 8; y++) {
-                        if constexpr (decltype(key_tag)::value) h[y] = h2_fma(h[y], f_hi, h2_mul(h[y], f_lo));
-                        else h[y] = h2_mul(h[y], f_hi);
-                    }
-                    *reinterpret_cast<uint4 *>(tile + f16_chunk_at(32 * w + row, 2 * c)) = make_uint4(h[0], h[1], h[2], h[3]);
-                    *reinterpret_cast<uint4 *>(tile + f16_chunk_at(32 * w + row, 2 * c + 1)) = make_uint4(h[4], h[5], h[6], h[7]);
-                }
-            };
-            if (keys) convert(std::true_type{});
-            else convert(std::false_type{});
+            for (int x = 0; x < N; x++) {
+                const int row = x * RPI + lane / CH;
+                const uint4 u = *reinterpret_cast<const uint4 *>(raw + row * HD + 16 * c);
+                uint32_t h[8];
+                codes_to_f16(u.x, h[0], h[1]);
+                codes_to_f16(u.y, h[2], h[3]);
+                codes_to_f16(u.z, h[4], h[5]);
+                codes_to_f16(u.w, h[6], h[7]);
+                *reinterpret_cast<uint4 *>(tile + f16_chunk_at(32 * w + row, 2 * c)) = make_uint4(h[0], h[1], h[2], h[3]);
+                *reinterpret_cast<uint4 *>(tile + f16_chunk_at(32 * w + row, 2 * c + 1)) = make_uint4(h[4], h[5], h[6], h[7]);
+            }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             mbar_arrive(&full[b]);
             if (j + 1 < n_tiles) ask(j + 1);
+            if (keys) publish();
         }
     } else {
         // ================= products =================

@@ -375,6 +375,11 @@ __device__ __forceinline__ float2 load_part2(const float2 *p) {
     asm volatile("ld.global.cg.v2.f32 {%0,%1}, [%2];" : "=f"(v.x), "=f"(v.y) : "l"(p) : "memory");
     return v;
 }
+// The consumer warps of a CTA.  bar.sync is .aligned: lanes that left a loop or a branch before the others meet them first.
+__device__ __forceinline__ void consumers_sync() {
+    __syncwarp();
+    named_barrier_sync(1, SH_THREADS);
+}
 struct Join {
     void *out;
     float *ws;
@@ -437,7 +442,7 @@ __device__ __noinline__ void join_parts(const Join &j) {     // not inlined: its
                 }
             }
         }
-        if (!j.last) named_barrier_sync(1, SH_THREADS);    // every thread has read the maxima and sums of slot `to` for its row
+        if (!j.last) consumers_sync();    // every thread has read the maxima and sums of slot `to` for its row
 #pragma unroll
         for (int e = 0; e < E; e++) {
             const int x = x0 + e * SH_THREADS;
@@ -458,14 +463,14 @@ __device__ __noinline__ void join_parts(const Join &j) {     // not inlined: its
 // Counts this CTA in; true in the one that completes `n`, which also clears the counter for the next launch.  The barrier
 // orders the CTA's writes before the count, whose release makes them visible to whoever counts later and acquires.
 __device__ __forceinline__ bool last_of(uint32_t *counter, uint32_t n, uint32_t *flag) {
-    named_barrier_sync(1, SH_THREADS);
+    consumers_sync();
     if (threadIdx.x == 0) {
         uint32_t before;
         asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(before) : "l"(counter) : "memory");
         if (before == n - 1) *counter = 0;
         *flag = before == n - 1;
     }
-    named_barrier_sync(1, SH_THREADS);
+    consumers_sync();
     return *flag != 0;
 }
 
@@ -515,6 +520,11 @@ attention_quant_short_kernel(const __grid_constant__ ShortMaps maps, const AttnQ
     if (warp >= SH_WARPS) {
         // ---- producer ----
         int issued = 0;
+        auto given = [&]() {                             // is the stage free?  All lanes go on or none does
+            dead = !__all_sync(0xffffffffu, mbar_wait(&empty[stage], phase ^ 1, polls));
+            if (dead && lane == 0) report_error(p.err, KERR_EMPTY_WAIT);
+            return !dead;
+        };
         while (!dead && walk.next(p, rows, s)) {
             const uint32_t *table = p.block_table + (size_t)s.req * p.max_blocks;
             if constexpr (TMA) {
@@ -530,7 +540,7 @@ attention_quant_short_kernel(const __grid_constant__ ShortMaps maps, const AttnQ
                     }
                     const int steps = min(32 / RUNS, s.n_steps - r0 / RUNS);
                     for (int i = 0; i < steps && !dead; i++) {
-                        if (issued >= NST && !mbar_wait(&empty[stage], phase ^ 1, polls)) { dead = true; report_error(p.err, KERR_EMPTY_WAIT); break; }
+                        if (issued >= NST && !given()) break;
                         uint8_t *cd = codes + stage * St::BYTES, *ax = aux + stage * St::AUX;
                         if (lane / RUNS == i) reinterpret_cast<uint32_t *>(ax + St::MASK)[lane % RUNS] = (1u << n_ok) - 1;
                         __syncwarp();
@@ -560,7 +570,7 @@ attention_quant_short_kernel(const __grid_constant__ ShortMaps maps, const AttnQ
                 };
                 uint32_t page[2] = {page_of(0, 2 * pw / HW), page_of(0, (2 * pw + 1) / HW)};
                 for (int i = 0; i < s.n_steps; i++) {
-                    if (issued >= NST && !mbar_wait(&empty[stage], phase ^ 1, polls)) { dead = true; report_error(p.err, KERR_EMPTY_WAIT); break; }
+                    if (issued >= NST && !given()) break;
                     uint8_t *cd = codes + stage * St::BYTES, *ax = aux + stage * St::AUX;
 #pragma unroll
                     for (int y = 0; y < 2; y++) {
@@ -656,6 +666,7 @@ attention_quant_short_kernel(const __grid_constant__ ShortMaps maps, const AttnQ
 
         for (int i = 0; i < s.n_steps; i++) {
             if (!dead && !mbar_wait(&full[stage], phase, polls)) { dead = true; report_error(p.err, KERR_FULL_WAIT); }
+            __syncwarp();                                // what follows is .aligned
             uint8_t *kt = codes + stage * St::BYTES + first_tile * 16 * HD, *vt = kt + St::TILE;
             const uint8_t *ax = aux + stage * St::AUX;
             const int p0 = (s.t0 + i) * TP + wp * 16 * GR;
@@ -838,7 +849,7 @@ attention_quant_short_kernel(const __grid_constant__ ShortMaps maps, const AttnQ
             float2 *ml = reinterpret_cast<float2 *>(meet + SH_WARPS * RB * D);
 #pragma unroll
             for (int c0 = 0; c0 < CH; c0 += PASS) {
-                named_barrier_sync(1, SH_THREADS);       // what was there has been read
+                consumers_sync();       // what was there has been read
 #pragma unroll
                 for (int n = 0; n < NT; n++)
 #pragma unroll
@@ -850,7 +861,7 @@ attention_quant_short_kernel(const __grid_constant__ ShortMaps maps, const AttnQ
                                 make_float2(o[n][c0 + c][e] * back, o[n][c0 + c][2 + e] * back);
                         if (g == 0) ml[warp * RB + i] = make_float2(m[n][e], l[n][e]);
                     }
-                named_barrier_sync(1, SH_THREADS);
+                consumers_sync();
                 for (int x = tid; x < HW * s.n_rows * (D / 4); x += SH_THREADS) {
                     const int d = 4 * (x % (D / 4)), i = x / (D / 4) % s.n_rows, hd = x / (D / 4) / s.n_rows;
                     float mm = -INFINITY;
@@ -1072,8 +1083,11 @@ attention_quant_long_kernel(const AttnQuant p, int skip_short, int span, uint32_
     tc_fence_after();
     const uint32_t tmem = tmem_base_s;                   // scores of tile t at 128 t, O at 256 + 128 t
     bool dead = false;
-    auto wait = [&](uint64_t *bar, uint32_t parity, uint32_t code) {     // gives up once; then nothing is waited for any more
+    // A whole warp: gives up once; then nothing is waited for any more.  Lanes leave the polling each for itself, and what follows
+    // (tcgen05.ld / st, bar.sync) is .aligned: the warp has to have met again.
+    auto wait = [&](uint64_t *bar, uint32_t parity, uint32_t code) {
         if (!dead && !mbar_wait(bar, parity, polls)) { dead = true; report_error(p.err, code); }
+        __syncwarp();
     };
 
     if (warp < 8) {
@@ -1200,7 +1214,7 @@ attention_quant_long_kernel(const AttnQuant p, int skip_short, int span, uint32_
                         uint32_t bits = 0;
                         if constexpr (MASKED) {
                             bits = bits_of(c >> 1);
-                            bad = bad || (bits & fl.bad[c >> 1]) != 0;
+                            bad |= (bits & fl.bad[c >> 1]) != 0;
                             bits >>= 16 * (c & 1);
                         }
 #pragma unroll
@@ -1235,6 +1249,7 @@ attention_quant_long_kernel(const AttnQuant p, int skip_short, int span, uint32_
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(&sc_empty[st]);
+            __syncwarp();
         }
         // ---- O, divided by the sum ----
         const float l = l2.x + l2.y;
@@ -1251,19 +1266,21 @@ attention_quant_long_kernel(const AttnQuant p, int skip_short, int span, uint32_
                 tmem_ld32(o_col + 32 * c, v);
                 tmem_ld_wait();
             }
-            if (!on) continue;
+            if (on) {                                    // not so for all lanes of a warp that the rows end in
 #pragma unroll
-            for (int x = 0; x < 32; x += 8) {
-                uint32_t h[4];
+                for (int x = 0; x < 32; x += 8) {
+                    uint32_t h[4];
 #pragma unroll
-                for (int y = 0; y < 4; y++) {
-                    // rows without positions: zeros (their columns of O may never have been written)
-                    const float a = len > 0 ? __uint_as_float(v[x + 2 * y]) * norm : 0.0f, b = len > 0 ? __uint_as_float(v[x + 2 * y + 1]) * norm : 0.0f;
-                    const __nv_bfloat162 z = __floats2bfloat162_rn(a, b);
-                    h[y] = *reinterpret_cast<const uint32_t *>(&z);
+                    for (int y = 0; y < 4; y++) {
+                        // rows without positions: zeros (their columns of O may never have been written)
+                        const float a = len > 0 ? __uint_as_float(v[x + 2 * y]) * norm : 0.0f, b = len > 0 ? __uint_as_float(v[x + 2 * y + 1]) * norm : 0.0f;
+                        const __nv_bfloat162 z = __floats2bfloat162_rn(a, b);
+                        h[y] = *reinterpret_cast<const uint32_t *>(&z);
+                    }
+                    *reinterpret_cast<uint4 *>(out + 32 * c + x) = make_uint4(h[0], h[1], h[2], h[3]);
                 }
-                *reinterpret_cast<uint4 *>(out + 32 * c + x) = make_uint4(h[0], h[1], h[2], h[3]);
             }
+            __syncwarp();
         }
         tc_fence_before();
     } else if (warp < 16) {
@@ -1333,6 +1350,7 @@ attention_quant_long_kernel(const AttnQuant p, int skip_short, int span, uint32_
                         top_s[b][w] = __float_as_uint(top);
                         look_s[b][w] = there != 0xFFFFFFFFu || bad;      // positions past kv_end, on a page beyond the pool, or marked
                     }
+                    __syncwarp();
                     named_barrier_sync(2, 128);          // what the four warps have found
                     const uint32_t most = max(max(top_s[b][0], top_s[b][1]), max(top_s[b][2], top_s[b][3]));
                     power = max(power, min((most + 0x7FFFFFu) & 0x7F800000u, 253u << 23));

@@ -118,3 +118,18 @@ def test_keys_of_all_sizes(backend, hd, news):
         q = (rand(news, nh * hd, seed=451, loud=False) * 2.0 ** -e).to(torch.bfloat16)
         out = attend(backend, q, kc, ks, vc, vs, table, [l], [news], nh, nkv, hd, block, most)
         check(out, *wanted(q, kc, ks, vc, vs, slots[0], news, nh, nkv, hd), l, torch.bfloat16)
+
+
+@pytest.mark.parametrize("group,tokens", [(1, 65), (3, 11), (4, 33), (5, 27), (7, 19), (8, 17), (17, 5), (32, 1)])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_row_counts_that_end_inside_a_warp(backend, hd, group, tokens):
+    """Rows (token x head of the group) that fill no whole warp of 32, beside a second request, with tokens behind the last: the
+    rows past the end are left as they were."""
+    nkv, block, lens, news = 2, 16, [200, 150], [tokens, 1]
+    nh = group * nkv
+    kc, ks, vc, vs, table, slots, most = paged_cache(nkv, hd, lens, block, 460)
+    q = rand(tokens + 3, nh * hd, seed=461, loud=False).to(torch.bfloat16)
+    out = attend(backend, q, kc, ks, vc, vs, table, lens, news, nh, nkv, hd, block, most)
+    check(out[:tokens], *wanted(q[:tokens], kc, ks, vc, vs, slots[0], tokens, nh, nkv, hd), lens[0], torch.bfloat16)
+    check(out[tokens:tokens + 1], *wanted(q[tokens:tokens + 1], kc, ks, vc, vs, slots[1], 1, nh, nkv, hd), lens[1], torch.bfloat16)
+    assert (out[tokens + 1:] == 7.0).all()

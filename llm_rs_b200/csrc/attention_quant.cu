@@ -177,8 +177,13 @@ __global__ void __launch_bounds__(AQ_TILE) attention_quant_simple_kernel(const A
 // product for what would take two the other way round; the weights change sides by movmatrix.  The order in
 // which dimensions enter a dot product is free as long as both operands agree, so a lane takes 16 consecutive codes
 // of a row as its part of four products; codes of values come transposed by ldmatrix in pairs of dimensions, which
-// one byte permute turns into pairs of positions.  A weight enters as w = e^(s - m) vs / R * 2^15 with R the least power
-// of two that no vs so far exceeds: f16 keeps it to 2^-11 (bf16: 2^-8), and down to 2^-40 of the largest.
+// one byte permute turns into pairs of positions.
+//
+// A weight enters as w = e^s vs / 2^a * 2^15, where a is the row's own: at least the largest s + log2 vs among the positions
+// that it has seen, and at most 10 more, so f16 keeps a weight to 2^-11 (bf16: 2^-8), and down to 2^-30 of the largest, whatever
+// other rows see and however large a value of little weight is.  Where the vs of the 32 positions
+// of a step lie within 2^10 of one another, the largest s of the row plus log2 of the largest vs does for a, and one exponential
+// does for the weight and the sum; elsewhere a is found position by position, and a weight has an exponential of its own.
 constexpr int SH_WARPS = 4, SH_THREADS = 32 * SH_WARPS;      // consumers
 constexpr int SH_GR = 2;             // runs of 16 positions that a warp takes at a time
 constexpr int SH_TILES = SH_WARPS * SH_GR;                   // (run, head) tiles of a unit
@@ -318,6 +323,10 @@ __device__ __forceinline__ int row_exponent(float amax) {
     const int e = (int)(__float_as_uint(amax) >> 23);    // biased; amax >= 0
     return amax == 0.0f || e == 255 ? 0 : max(-126, min(126, 13 - (e - 127)));
 }
+// Powers of two, as a float's bits: the one at or below a size, the least that it does not exceed; between 2^-126 and 2^126.
+__device__ __forceinline__ uint32_t power_of(float size) { return max(1u << 23, min(__float_as_uint(size) & 0x7F800000u, 253u << 23)); }
+__device__ __forceinline__ uint32_t power_above(float size) { return max(1u << 23, min((__float_as_uint(size) + 0x7FFFFFu) & 0x7F800000u, 253u << 23)); }
+__device__ __forceinline__ float log2_of(uint32_t power_bits) { return (float)((int)(power_bits >> 23) - 127); }
 // 16-byte chunk c of row `row` of a tile of HD-byte rows, as the 128- and 64-byte swizzles of TMA place it.
 template <int HD> __device__ __forceinline__ int chunk_at(int row, int c) {
     return row * HD + 16 * (c ^ (HD == 128 ? row & 7 : (row >> 1) & 3));
@@ -654,16 +663,14 @@ attention_quant_short_kernel(const __grid_constant__ ShortMaps maps, const AttnQ
         }
         // [rows 8n ..][chunk of 16 dims]: dims 16c + 2g (0, 1) and 16c + 2g + 1 (2, 3) of rows 2t (0, 2) and 2t + 1 (1, 3)
         float o[NT][CH][4];
-        float m[NT][2], l[NT][2];
+        float m[NT][2], l[NT][2], a[NT][2];              // O counts in 2^(a - 15)
 #pragma unroll
         for (int n = 0; n < NT; n++) {
-            m[n][0] = m[n][1] = -INFINITY;
+            m[n][0] = m[n][1] = a[n][0] = a[n][1] = -INFINITY;
             l[n][0] = l[n][1] = 0.0f;
 #pragma unroll
             for (int c = 0; c < CH; c++) o[n][c][0] = o[n][c][1] = o[n][c][2] = o[n][c][3] = 0.0f;
         }
-        uint32_t r_bits = 17u << 23;                     // R: a power of two, at least 2^-110
-
         for (int i = 0; i < s.n_steps; i++) {
             if (!dead && !mbar_wait(&full[stage], phase, polls)) { dead = true; report_error(p.err, KERR_FULL_WAIT); }
             __syncwarp();                                // what follows is .aligned
@@ -704,7 +711,7 @@ attention_quant_short_kernel(const __grid_constant__ ShortMaps maps, const AttnQ
                     }
                 }
             }
-            // ---- what a row does not see, the running maxima, the size of the values, the weights ----
+            // ---- what a row does not see, the running maxima, the sizes of what is summed, the weights ----
 #pragma unroll
             for (int r = 0; r < GR; r++)
 #pragma unroll
@@ -733,14 +740,24 @@ attention_quant_short_kernel(const __grid_constant__ ShortMaps maps, const AttnQ
                 }
                 __syncwarp();
             }
-            float vmax = 0.0f;
+            float vmax = 0.0f, av[GR][2];                // sizes of the values' scales (0: not finite)
 #pragma unroll
-            for (int r = 0; r < GR; r++) vmax = fmaxf(vmax, fmaxf(vw[r][0], vw[r][1]));
+            for (int r = 0; r < GR; r++)
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    av[r][h] = fabsf(vw[r][h]) <= 3.402823466e38f ? fabsf(vw[r][h]) : 0.0f;
+                    vmax = fmaxf(vmax, av[r][h]);
+                }
 #pragma unroll
             for (int x = 4; x <= 16; x <<= 1) vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, x));
-            const uint32_t r_new = max(r_bits, min((__float_as_uint(vmax) + 0x7FFFFFu) & 0x7F800000u, 253u << 23));
-            bool moved = r_new != r_bits;
-            float f[NT][2], top[NT][2];
+            const uint32_t v_bits = power_above(vmax);
+            const float v_log = log2_of(v_bits);
+            bool near = true;                            // those that are there are of sizes within 2^10 of one another
+#pragma unroll
+            for (int r = 0; r < GR; r++)
+#pragma unroll
+                for (int h = 0; h < 2; h++) near = near && (av[r][h] >= __uint_as_float(v_bits) * 0x1p-10f || !(mask[r] >> (g + 8 * h) & 1));
+            float mn[NT][2], an[NT][2], top[NT][2], ref[NT][2];          // the new m and a; m and what scores count from, finite
 #pragma unroll
             for (int n = 0; n < NT; n++)
 #pragma unroll
@@ -750,47 +767,82 @@ attention_quant_short_kernel(const __grid_constant__ ShortMaps maps, const AttnQ
                     for (int r = 1; r < GR; r++) mx = fmaxf(mx, fmaxf(sc[r][n][e], sc[r][n][2 + e]));
 #pragma unroll
                     for (int x = 4; x <= 16; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
-                    const float mn = fmaxf(m[n][e], mx);
-                    top[n][e] = mn == -INFINITY ? 0.0f : mn;             // a row that has seen nothing yet
-                    f[n][e] = mn == m[n][e] ? 1.0f : ex2(m[n][e] - top[n][e]);
-                    m[n][e] = mn;
-                    moved = moved || f[n][e] != 1.0f;
+                    mn[n][e] = fmaxf(m[n][e], mx);
+                    an[n][e] = fmaxf(a[n][e], mx + v_log);               // at least the largest s + log2 vs that the row sees
+                    top[n][e] = mn[n][e] == -INFINITY ? 0.0f : mn[n][e]; // a row that has seen nothing yet
+                    ref[n][e] = (an[n][e] == -INFINITY ? 0.0f : an[n][e]) - (15.0f + v_log);
+                    near = near && ref[n][e] - top[n][e] <= 80.0f;       // the sum keeps its weights above float32's least
                 }
-            if (__any_sync(0xffffffffu, moved)) {
-                const float sh = r_new - r_bits >= (127u << 23) ? 0.0f : __uint_as_float(r_bits - r_new + (127u << 23));      // R / R'
+            near = __all_sync(0xffffffffu, near);
+            if (!near) {
 #pragma unroll
                 for (int n = 0; n < NT; n++)
 #pragma unroll
                     for (int e = 0; e < 2; e++) {
-                        l[n][e] *= f[n][e];
-                        const float x = f[n][e] * sh;
+                        float mv = -INFINITY;
 #pragma unroll
-                        for (int c = 0; c < CH; c++) { o[n][c][e] *= x; o[n][c][2 + e] *= x; }
+                        for (int r = 0; r < GR; r++)
+#pragma unroll
+                            for (int h = 0; h < 2; h++)
+                                if (av[r][h] > 0.0f) mv = fmaxf(mv, sc[r][n][2 * h + e] + log2_of(power_above(av[r][h])));
+#pragma unroll
+                        for (int x = 4; x <= 16; x <<= 1) mv = fmaxf(mv, __shfl_xor_sync(0xffffffffu, mv, x));
+                        an[n][e] = fmaxf(a[n][e], mv);
+                        ref[n][e] = an[n][e] == -INFINITY ? 0.0f : an[n][e];
                     }
-                r_bits = r_new;
             }
-            const float inv_r = __uint_as_float(((127u + 127u + 15u) << 23) - r_bits);   // 2^15 / R
-            uint32_t pb[TERMS][GR][NT][2];
+            bool moved = false;
 #pragma unroll
-            for (int r = 0; r < GR; r++)
+            for (int n = 0; n < NT; n++)
 #pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    const float vr = vw[r][h] * inv_r;
+                for (int e = 0; e < 2; e++) moved = moved || mn[n][e] != m[n][e] || an[n][e] != a[n][e];
+            if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
-                    for (int n = 0; n < NT; n++) {
-                        float w[2];
+                for (int n = 0; n < NT; n++)
 #pragma unroll
-                        for (int e = 0; e < 2; e++) {
-                            const float x = ex2(sc[r][n][2 * h + e] - top[n][e]);
-                            l[n][e] += x;
-                            w[e] = x * vr;
-                            if (!all && sc[r][n][2 * h + e] == -INFINITY) w[e] = 0.0f;          // not 0 * NaN
-                        }
-                        const uint32_t hi = pack_f16(w[0], w[1]);
-                        pb[0][r][n][h] = transposed(hi);
-                        if (TERMS == 2) pb[TERMS - 1][r][n][h] = transposed(pack_f16_rest(w[0], w[1], hi));
+                    for (int e = 0; e < 2; e++) {
+                        if (mn[n][e] != m[n][e]) l[n][e] *= ex2(m[n][e] - mn[n][e]);
+                        const float f = an[n][e] == a[n][e] ? 1.0f : ex2(a[n][e] - an[n][e]);
+#pragma unroll
+                        for (int c = 0; c < CH; c++) { o[n][c][e] *= f; o[n][c][2 + e] *= f; }
+                        m[n][e] = mn[n][e];
+                        a[n][e] = an[n][e];
                     }
-                }
+            }
+            uint32_t pb[TERMS][GR][NT][2];
+            auto weights = [&](auto near_tag) {
+                constexpr bool NEAR = decltype(near_tag)::value;
+                float sum[NT][2];
+#pragma unroll
+                for (int n = 0; n < NT; n++) sum[n][0] = sum[n][1] = 0.0f;
+#pragma unroll
+                for (int r = 0; r < GR; r++)
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        const uint32_t by = NEAR ? v_bits : power_of(av[r][h]);  // a value by itself: vs = 2^own times its rest
+                        const float vr = vw[r][h] * __uint_as_float((254u << 23) - by), own = 15.0f + log2_of(by);
+#pragma unroll
+                        for (int n = 0; n < NT; n++) {
+                            float w[2];
+#pragma unroll
+                            for (int e = 0; e < 2; e++) {
+                                // (scores and references, large numbers that are alike, are subtracted before anything else: that is exact)
+                                const float score = sc[r][n][2 * h + e], x = ex2(score - (NEAR ? ref[n][e] : top[n][e]));
+                                sum[n][e] += x;
+                                w[e] = NEAR ? x * vr : score == -INFINITY ? 0.0f : ex2((score - ref[n][e]) + own) * vr;      // not 0 * NaN
+                            }
+                            const uint32_t hi = pack_f16(w[0], w[1]);
+                            pb[0][r][n][h] = transposed(hi);
+                            if (TERMS == 2) pb[TERMS - 1][r][n][h] = transposed(pack_f16_rest(w[0], w[1], hi));
+                        }
+                    }
+#pragma unroll
+                for (int n = 0; n < NT; n++)
+#pragma unroll
+                    for (int e = 0; e < 2; e++) l[n][e] += NEAR ? sum[n][e] * ex2(ref[n][e] - top[n][e]) : sum[n][e];
+            };
+            if (near) weights(std::true_type{});
+            else weights(std::false_type{});
             // ---- weighted values: 16 dimensions a product ----
 #pragma unroll
             for (int r = 0; r < GR; r++)
@@ -815,7 +867,15 @@ attention_quant_short_kernel(const __grid_constant__ ShortMaps maps, const AttnQ
             if (++stage == NST) { stage = 0; phase ^= 1; }
         }
         // ---- the row block's part is done: out, or into the workspace ----
-        const float back = __uint_as_float(r_bits - (15u << 23));        // R / 2^15
+        float back[NT][2][2];                            // 2^(a - 15 - m), in two factors: each stays in float32's range
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                const float x = a[n][e] == -INFINITY ? -INFINITY : (a[n][e] - m[n][e]) - 15.0f, y = truncf(0.5f * x);
+                back[n][e][0] = x == -INFINITY ? 0.0f : ex2(y);
+                back[n][e][1] = x == -INFINITY ? 0.0f : ex2(x - y);
+            }
         const bool whole = s.t0 == 0 && s.t1 == s.tiles;
         const int slot = blockIdx.x * 2 + (s.first ? 0 : 1);
         float *ws_o = ws + (size_t)slot * HW * RB * HD;
@@ -833,11 +893,11 @@ attention_quant_short_kernel(const __grid_constant__ ShortMaps maps, const AttnQ
                 for (int e = 0; e < 2; e++) {
                     const int i = 8 * n + 2 * t + e, rr = s.rb * RB + i;
                     if (i >= s.n_rows) continue;
-                    const float norm = whole ? (l[n][e] == 0.0f ? 0.0f : back / l[n][e]) : back;
+                    const float b0 = back[n][e][0], b1 = whole ? (l[n][e] == 0.0f ? 0.0f : back[n][e][1] / l[n][e]) : back[n][e][1];
                     const size_t off = ((size_t)(s.r.first + rr / group) * p.n_heads + (size_t)kvh * group + rr % group) * HD;
 #pragma unroll
                     for (int c = 0; c < CH; c++) {
-                        const float2 v = make_float2(o[n][c][e] * norm, o[n][c][2 + e] * norm);
+                        const float2 v = make_float2(o[n][c][e] * b0 * b1, o[n][c][2 + e] * b0 * b1);
                         if (whole) store2(p.out, off + 16 * c + 2 * g, v, bf16);
                         else *reinterpret_cast<float2 *>(ws_o + ((size_t)hw * RB + i) * HD + 16 * c + 2 * g) = v;
                     }
@@ -858,7 +918,7 @@ attention_quant_short_kernel(const __grid_constant__ ShortMaps maps, const AttnQ
 #pragma unroll
                         for (int c = 0; c < PASS; c++)
                             *reinterpret_cast<float2 *>(meet + ((size_t)warp * RB + i) * D + 16 * c + 2 * g) =
-                                make_float2(o[n][c0 + c][e] * back, o[n][c0 + c][2 + e] * back);
+                                make_float2(o[n][c0 + c][e] * back[n][e][0] * back[n][e][1], o[n][c0 + c][2 + e] * back[n][e][0] * back[n][e][1]);
                         if (g == 0) ml[warp * RB + i] = make_float2(m[n][e], l[n][e]);
                     }
                 consumers_sync();

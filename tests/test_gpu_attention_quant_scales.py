@@ -93,9 +93,9 @@ OUTLIERS = [2.0 ** 24, 2.0 ** 40, 2.0 ** 90, math.inf, math.nan]
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
-@pytest.mark.parametrize("which", ["keys"])
 @pytest.mark.parametrize("size", OUTLIERS)
-@pytest.mark.parametrize("hd,news", [(64, 4), (128, 3), (64, 70), (128, 150), (96, 20)])
+@pytest.mark.parametrize("which,hd,news", [("keys", 64, 4), ("keys", 128, 3), ("keys", 64, 70), ("keys", 128, 150), ("keys", 96, 20),
+                                           ("values", 64, 4), ("values", 128, 3), ("values", 96, 20)])
 def test_positions_that_a_row_does_not_see_do_not_show(backend, hd, news, size, which, dtype):
     """The last position, which only the last token sees, has a scale that is larger than the others by `size`."""
     nh, nkv, block, l = 8, 2, 16, 300
@@ -106,6 +106,41 @@ def test_positions_that_a_row_does_not_see_do_not_show(backend, hd, news, size, 
     want = wanted(q, kc, ks, vc, vs, slots[0], news, nh, nkv, hd)
     rows = slice(0, news - 1)
     check(out[rows], *(x[rows] for x in want), l, dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("hd,news", [(64, 1), (128, 1), (128, 4), (96, 2)])
+@pytest.mark.parametrize("at,size,depth", [(0, 2.0 ** 30, 300.0), (37, 2.0 ** 45, 300.0), (399, 2.0 ** 30, 300.0), (500, 2.0 ** 60, 300.0),
+                                           (250, 2.0 ** 29, 20.0), (0, 2.0 ** 40, 20.0), (699, 2.0 ** 20, 40.0)])
+def test_large_values_count_by_their_share(backend, hd, news, at, size, depth, dtype):
+    """A position that is seen by every row (the last one: by the last) has a value `size` times the others and a score `depth`
+    below them: what it adds is e^-depth of it, nothing at 300 (2^-433), about as much as the others at 20 and 2^29."""
+    nh, nkv, block, l = 8, 2, 16, 700
+    kc, ks, vc, vs, table, slots, most = paged_cache(nkv, hd, [l], block, 430)
+    q = rand(news, nh * hd, seed=431, loud=False).view(news, nh, hd)
+    q[..., 0] = 4.0
+    k = rand(l, nkv * hd, seed=432, loud=False).view(l, nkv, hd)
+    k[at, :, :] = 0.0
+    k[at, :, 0] = -depth / 4.0 * math.sqrt(hd)
+    q = q.view(news, -1).to(dtype)
+    kc[slots[0]], ks[:, slots[0]] = quantised(k.view(l, -1), nkv)
+    vs[:, slots[0][at]] *= size
+    out = attend(backend, q, kc, ks, vc, vs, table, [l], [news], nh, nkv, hd, block, most)
+    check(out, *wanted(q, kc, ks, vc, vs, slots[0], news, nh, nkv, hd), l, dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("hd,news", [(64, 1), (128, 4), (96, 2)])
+@pytest.mark.parametrize("low,high", [(-20, 20), (-60, 60), (-120, -80), (60, 100)])
+def test_scales_of_all_sizes(backend, hd, news, low, high, dtype):
+    """Values whose scales are spread evenly over many powers of two, position by position."""
+    nh, nkv, block, l = 8, 2, 16, 700
+    kc, ks, vc, vs, table, slots, most = paged_cache(nkv, hd, [l], block, 440)
+    g = torch.Generator().manual_seed(441)
+    vs[:, slots[0]] = torch.exp2(torch.rand(nkv, l, generator=g) * (high - low) + low).cuda()
+    q = rand(news, nh * hd, seed=442, loud=False).to(dtype)
+    out = attend(backend, q, kc, ks, vc, vs, table, [l], [news], nh, nkv, hd, block, most)
+    check(out, *wanted(q, kc, ks, vc, vs, slots[0], news, nh, nkv, hd), l, dtype)
 
 
 @pytest.mark.parametrize("hd,news", [(64, 1), (128, 4), (128, 50)])

@@ -986,15 +986,19 @@ attention_quant_short_kernel(const __grid_constant__ ShortMaps maps, const AttnQ
 //   warp 16          issues the products: S = Q K^T (both from shared memory), O += W V (W from TMEM; the values lie
 //                    as they come, positions in rows, so they are the operand's major dimension the other way round).
 //
-// Softmax in one pass: O and the sum refer to a maximum that is only moved when a row's grows by more than 6 (log2), so O
-// is rarely rescaled (2 instead of 6: 4096 tokens 207 us instead of 191); weights then stay below 64, and enter as
-// e^(s - m) * 2^9: f16 keeps 2^-11 of a weight, and down to 2^-34 of the largest.
+// Softmax in one pass.  The sum refers to a maximum m of the row's scores and O to a of its s + log2 vs, both only moved when
+// outgrown by more than 6 (log2), so O is rarely rescaled (2 instead of 6: 4096 tokens 207 us instead of 191, at that step).
+// Weights enter as e^s vs / 2^a * 2^9, below 2^15: f16 keeps 2^-11 of a weight.
 //
-// The codes, exact in f16, are what is multiplied; ks enters at the score and vs / R at the weight, in float32 (R as in the other
-// kernel).  Multiplied into the f16 keys and values instead, once a code and not once a score, they make the weights 1.75
-// instructions a score shorter (4096 tokens 200 us instead of 242), but every product is then rounded to 2^-11: a weight
-// behind a score of 300 is off by a tenth.  A value whose scale is not finite is zero there, and the rows that see it are marked,
-// so that no row sees NaN times zero.
+// The codes, exact in f16, are what is multiplied; ks enters at the score and vs at the weight, in float32.  Multiplied
+// into the f16 keys and values instead, once a code and not once a score, they make the weights 1.75 instructions a score
+// shorter (4096 tokens 200 us instead of 242), but every product is then rounded to 2^-11: a weight behind a score of 300
+// is off by a tenth.
+//
+// Only what a row sees decides its references.  In a tile of positions whose vs lie within 2^10 of one another the row's largest
+// score plus log2 of the tile's largest vs does for a, at most 10 too much, so f16 keeps a weight down to 2^-24 of the largest; in
+// others a is found position by position, and a weight has an exponential of its own.  A value whose scale is not finite is zero
+// there, and the rows that see it are marked, so that no row sees NaN times zero.
 constexpr int LG_ROWS = 128, LG_POS = 128, LG_THREADS = 17 * 32;
 constexpr float LG_SLACK = 6.0f;     // log2: the weights' factor 2^9 leaves these octaves to f16's 65504
 
@@ -1002,12 +1006,14 @@ struct LongFlags {                   // of a tile of positions, 32 to a warp
     uint32_t there[4];               // which of them are
     uint32_t bad[4];                 // whose value's scale is not finite
     uint32_t big[4];                 // whose key's scale is above 2^90
-    uint32_t all, r_bits;            // nothing of this needs a look; R
+    uint32_t wide[4];                // whose value's scale is below 2^-10 of the tile's largest
+    uint32_t all;                    // are there, and none of them bad
+    float v_log, v_unit;             // log2 of a power of two that no value's scale exceeds, and of the unit of those in VW
 };
 template <int HD> struct LongSmem {
     static constexpr int HALVES = HD / 64, TILE = LG_ROWS * HD * 2;      // 128 rows of f16, in halves of 64 dimensions
     static constexpr int Q = 0, K = 2 * TILE, V = K + 2 * TILE, RAW = V + 2 * TILE, SC = RAW + 2 * (TILE / 2);
-    static constexpr int STAGES = 2, KS = 0, VW = 512, SCALES = 1024;    // of a tile of positions: ks [128], vs / R [128]
+    static constexpr int STAGES = 2, KS = 0, VW = 512, SCALES = 1024;    // of a tile of positions: ks [128], vs / 2^v_unit [128]
     static constexpr int BYTES = SC + STAGES * SCALES;
 };
 
@@ -1075,7 +1081,8 @@ attention_quant_long_kernel(const AttnQuant p, int skip_short, int span, uint32_
     extern __shared__ __align__(1024) uint8_t lg_smem[];
     __shared__ __align__(8) uint64_t q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], sc_full[Sm::STAGES], sc_empty[Sm::STAGES], s_full[2], p_full[2], o_full[2];
     __shared__ LongFlags flags_s[Sm::STAGES];
-    __shared__ uint32_t tmem_base_s, top_s[2][4], look_s[2][4];
+    __shared__ uint32_t tmem_base_s, look_s[2][4];
+    __shared__ float top_s[2][4];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if (tid == 0) {
         for (int i = 0; i < 2; i++) {
@@ -1184,9 +1191,7 @@ attention_quant_long_kernel(const AttnQuant p, int skip_short, int span, uint32_
 
         const uint32_t lane_base = tmem + ((uint32_t)(warp & 3) << 21);          // this warp's 32 lanes
         const uint32_t s_col = lane_base + 128 * t, o_col = lane_base + 256 + 128 * t;
-        float m_ref = -INFINITY;
-        float2 l2 = make_float2(0.0f, 0.0f);
-        uint32_t r_bits = 17u << 23;
+        float m_ref = -INFINITY, a_ref = -INFINITY, l = 0.0f;            // the sum counts in 2^m_ref, O in 2^(a_ref - 9)
         for (int j = 0; j < n_tiles; j++) {
             const int st = j % Sm::STAGES;
             wait(&sc_full[st], (j / Sm::STAGES) & 1, KERR_FULL_WAIT);
@@ -1194,8 +1199,8 @@ attention_quant_long_kernel(const AttnQuant p, int skip_short, int span, uint32_
                 const uint8_t *sc = lg_smem + Sm::SC + st * Sm::SCALES;
                 const float *ks = reinterpret_cast<const float *>(sc + Sm::KS), *vw = reinterpret_cast<const float *>(sc + Sm::VW);
                 const LongFlags &fl = flags_s[st];
-                const uint32_t r_new = fl.r_bits;
-                const bool masked = !full_tile || (j + 1) * LG_POS > min_len || fl.all == 0 || (fl.big[0] | fl.big[1] | fl.big[2] | fl.big[3]) != 0;
+                const bool wide = (fl.wide[0] | fl.wide[1] | fl.wide[2] | fl.wide[3] | fl.big[0] | fl.big[1] | fl.big[2] | fl.big[3]) != 0;
+                const bool masked = !full_tile || (j + 1) * LG_POS > min_len || fl.all == 0 || wide;
                 wait(&s_full[t], j & 1, KERR_MMA_WAIT);
                 tc_fence_after();
                 auto bits_of = [&](int c) -> uint32_t {  // which of the 32 positions of chunk c this row sees
@@ -1203,20 +1208,15 @@ attention_quant_long_kernel(const AttnQuant p, int skip_short, int span, uint32_
                     const uint32_t there = fl.there[c];
                     return n <= 0 ? 0u : n >= 32 ? there : there & ((1u << n) - 1);
                 };
-                // Two forms of the code, chosen by the warp: most tiles are seen by every row whole, and a test a score costs
-                // more than the score's own arithmetic.  Each 16 columns are asked for while the 16 before are worked on.
-                auto work = [&](auto mask_tag) {
-                    constexpr bool MASKED = decltype(mask_tag)::value;
-                    uint32_t v[2][16];
-                    // A sum of codes and queries is below 2^30; times a scale of 2^98 it would leave float32 before the row's
-                    // factor brings it back, so the masked form multiplies scale and factor first.
-                    const float2 c2 = make_float2(c_row, c_row);
-                    auto scaled = [&](float a, float b, float ka, float kb) {
-                        const float2 k2 = MASKED ? pair_mul(make_float2(ka, kb), c2) : make_float2(ka, kb);
-                        return pair_mul(make_float2(a, b), k2);
-                    };
-                    // ---- the row's maximum ----
-                    float mx0 = -INFINITY, mx1 = -INFINITY;
+                // Three forms of the code, chosen by the warp: most tiles are seen by every row whole, and a test a score costs
+                // more than the score's own arithmetic (MASKED); scales that differ by much are rare (WIDE).  Each 16 columns are
+                // asked for while the 16 before are worked on.
+                uint32_t v[2][16];
+                const float2 c2 = make_float2(c_row, c_row);
+                float mx = -INFINITY, mv = -INFINITY;    // of what the row sees: the largest score, at least the largest s + log2 vs
+                auto largest = [&](auto mask_tag, auto wide_tag) {
+                    constexpr bool MASKED = decltype(mask_tag)::value, WIDE = decltype(wide_tag)::value;
+                    float mx1 = -INFINITY, mv1 = -INFINITY;
                     tmem_ld16(s_col, v[0]);
                     tmem_ld_wait();
 #pragma unroll
@@ -1228,43 +1228,63 @@ attention_quant_long_kernel(const AttnQuant p, int skip_short, int span, uint32_
 #pragma unroll
                         for (int x = 0; x < 16; x += 4) {
                             const float4 k4 = *reinterpret_cast<const float4 *>(ks + 16 * c + x);
-                            float2 a = scaled(__uint_as_float(u[x]), __uint_as_float(u[x + 1]), k4.x, k4.y);
-                            float2 d = scaled(__uint_as_float(u[x + 2]), __uint_as_float(u[x + 3]), k4.z, k4.w);
+                            float2 ka = make_float2(k4.x, k4.y), kb = make_float2(k4.z, k4.w);
+                            if constexpr (WIDE) {        // a sum of codes and queries, below 2^30, times a scale of 2^98 would leave float32
+                                ka = pair_mul(ka, c2);
+                                kb = pair_mul(kb, c2);
+                            }
+                            float2 a = pair_mul(make_float2(__uint_as_float(u[x]), __uint_as_float(u[x + 1])), ka);
+                            float2 d = pair_mul(make_float2(__uint_as_float(u[x + 2]), __uint_as_float(u[x + 3])), kb);
                             if constexpr (MASKED) {
                                 if (!(bits >> x & 1)) a.x = -INFINITY;
                                 if (!(bits >> (x + 1) & 1)) a.y = -INFINITY;
                                 if (!(bits >> (x + 2) & 1)) d.x = -INFINITY;
                                 if (!(bits >> (x + 3) & 1)) d.y = -INFINITY;
                             }
-                            mx0 = fmaxf(mx0, fmaxf(a.x, a.y));
+                            if constexpr (WIDE) {
+                                const float4 w4 = *reinterpret_cast<const float4 *>(vw + 16 * c + x);
+                                auto share = [&](float score, float vs) { return vs == 0.0f ? -INFINITY : score + log2_of(power_above(fabsf(vs))); };
+                                mv = fmaxf(mv, fmaxf(share(a.x, w4.x), share(a.y, w4.y)));
+                                mv1 = fmaxf(mv1, fmaxf(share(d.x, w4.z), share(d.y, w4.w)));
+                            }
+                            mx = fmaxf(mx, fmaxf(a.x, a.y));
                             mx1 = fmaxf(mx1, fmaxf(d.x, d.y));
                         }
                         tmem_ld_wait();
                     }
-                    const float mx = MASKED ? fmaxf(mx0, mx1) : fmaxf(mx0, mx1) * c_row;
-                    // ---- move the reference, O and the sum where the maximum has outgrown it ----
-                    const float m_new = mx > m_ref + LG_SLACK ? mx : m_ref;      // m_ref = -inf: any score at all
-                    const bool moved = m_new != m_ref || r_new != r_bits;
-                    const float base = m_new == -INFINITY ? 0.0f : m_new;
-                    if (j > 0 && __any_sync(0xffffffffu, moved)) {
-                        const float f = m_new == m_ref ? 1.0f : ex2(m_ref - base);
-                        const float sh = r_new - r_bits >= (127u << 23) ? 0.0f : __uint_as_float(r_bits - r_new + (127u << 23));      // R / R'
-                        l2.x *= f;
-                        l2.y *= f;
+                    mx = fmaxf(mx, mx1);
+                    if constexpr (!WIDE) mx *= c_row;
+                    mv = WIDE ? fmaxf(mv, mv1) + fl.v_unit : mx + fl.v_log;
+                };
+                if (!masked) largest(std::false_type{}, std::false_type{});
+                else if (!wide) largest(std::true_type{}, std::false_type{});
+                else largest(std::true_type{}, std::true_type{});
+                // ---- move the references, O and the sum where they have been outgrown ----
+                const float m_new = mx > m_ref + LG_SLACK ? mx : m_ref, a_new = mv > a_ref + LG_SLACK ? mv : a_ref;      // -inf: by any at all
+                const float m_base = m_new == -INFINITY ? 0.0f : m_new, a_base = a_new == -INFINITY ? 0.0f : a_new;
+                if (m_new != m_ref) l *= ex2(m_ref - m_base);
+                if (j > 0 && __any_sync(0xffffffffu, a_new != a_ref)) {
+                    const float f = a_new == a_ref ? 1.0f : ex2(a_ref - a_base);
 #pragma unroll
-                        for (int c = 0; c < HD / 16; c++) {
-                            uint32_t o[16];
-                            tmem_ld16(o_col + 16 * c, o);
-                            tmem_ld_wait();
+                    for (int c = 0; c < HD / 16; c++) {
+                        uint32_t o[16];
+                        tmem_ld16(o_col + 16 * c, o);
+                        tmem_ld_wait();
 #pragma unroll
-                            for (int x = 0; x < 16; x++) o[x] = __float_as_uint(__uint_as_float(o[x]) * (f * sh));
-                            tmem_st16(o_col + 16 * c, o);
-                        }
+                        for (int x = 0; x < 16; x++) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
+                        tmem_st16(o_col + 16 * c, o);
                     }
-                    m_ref = m_new;
-                    r_bits = r_new;
-                    // ---- the weights, over the scores ----
-                    const float2 nb = make_float2(9.0f - base, 9.0f - base), one2 = make_float2(1.0f, 1.0f);
+                }
+                m_ref = m_new;
+                a_ref = a_new;
+                // ---- the weights, over the scores ----
+                const float from = a_base - (9.0f + fl.v_unit);          // what the exponents of weights count from
+                // One exponential for weight and sum, unless what the sum gets would leave float32 below.
+                const bool apart = wide || __any_sync(0xffffffffu, from - m_base > 80.0f);
+                auto weights = [&](auto mask_tag, auto apart_tag) {
+                    constexpr bool MASKED = decltype(mask_tag)::value, APART = decltype(apart_tag)::value;
+                    const float2 nb = make_float2(-from, -from);
+                    float2 l2 = make_float2(0.0f, 0.0f);
                     bool bad = false;
                     uint32_t w[16];
 #pragma unroll
@@ -1283,26 +1303,37 @@ attention_quant_long_kernel(const AttnQuant p, int skip_short, int span, uint32_
 #pragma unroll
                             for (int y = 0; y < 2; y++) {
                                 const int at = x + 2 * y;
-                                float2 e = scaled(__uint_as_float(u[at]), __uint_as_float(u[at + 1]), y ? k4.z : k4.x, y ? k4.w : k4.y);
-                                e = MASKED ? pair_op(e, one2, nb) : pair_op(e, c2, nb);
-                                e.x = ex2(e.x);
-                                e.y = ex2(e.y);
+                                const float2 s2 = make_float2(__uint_as_float(u[at]), __uint_as_float(u[at + 1]));
+                                const float2 k2 = y ? make_float2(k4.z, k4.w) : make_float2(k4.x, k4.y), v2 = y ? make_float2(w4.z, w4.w) : make_float2(w4.x, w4.y);
+                                float2 e, z;             // what the sum gets, the weights
+                                if constexpr (APART) {
+                                    const float2 score = pair_mul(s2, pair_mul(k2, c2));
+                                    e = make_float2(ex2(score.x - m_base), ex2(score.y - m_base));
+                                    const uint32_t px = power_of(fabsf(v2.x)), py = power_of(fabsf(v2.y));       // vs = 2^p times its rest
+                                    z.x = ex2((score.x - from) + log2_of(px)) * (v2.x * __uint_as_float((254u << 23) - px));
+                                    z.y = ex2((score.y - from) + log2_of(py)) * (v2.y * __uint_as_float((254u << 23) - py));
+                                } else {
+                                    e = pair_op(pair_mul(s2, k2), c2, nb);
+                                    e = make_float2(ex2(e.x), ex2(e.y));
+                                }
                                 if constexpr (MASKED) {
-                                    if (!(bits >> at & 1)) e.x = 0.0f;
-                                    if (!(bits >> (at + 1) & 1)) e.y = 0.0f;
+                                    if (!(bits >> at & 1)) e.x = z.x = 0.0f;
+                                    if (!(bits >> (at + 1) & 1)) e.y = z.y = 0.0f;
                                 }
                                 l2 = pair_add(l2, e);
-                                e = pair_mul(e, y ? make_float2(w4.z, w4.w) : make_float2(w4.x, w4.y));
-                                w[8 * (c & 1) + at / 2] = pack_f16(e.x, e.y);
+                                if constexpr (!APART) z = pair_mul(e, v2);
+                                w[8 * (c & 1) + at / 2] = pack_f16(z.x, z.y);
                             }
                         }
                         if (c < 7) tmem_ld_wait();
                         if (c & 1) tmem_st16(s_col + 16 * (c >> 1), w);
                     }
-                    if (MASKED && bad) l2.x = __int_as_float(0x7FC00000);        // sees a value that is NaN
+                    l += APART ? l2.x + l2.y : (l2.x + l2.y) * ex2(from - m_base);
+                    if (MASKED && bad) l = __int_as_float(0x7FC00000);   // sees a value that is NaN
                 };
-                if (masked) work(std::true_type{});
-                else work(std::false_type{});
+                if (apart) weights(std::true_type{}, std::true_type{});
+                else if (masked) weights(std::true_type{}, std::false_type{});
+                else weights(std::false_type{}, std::false_type{});
                 tmem_st_wait();
                 tc_fence_before();
                 mbar_arrive(&p_full[t]);
@@ -1312,8 +1343,10 @@ attention_quant_long_kernel(const AttnQuant p, int skip_short, int span, uint32_
             __syncwarp();
         }
         // ---- O, divided by the sum ----
-        const float l = l2.x + l2.y;
-        const float norm = l == 0.0f ? 0.0f : __uint_as_float(r_bits) / l;
+        // 2^(a - 9 - m) / l in two factors: each stays in float32's range
+        const float back = (a_ref - m_ref) - 9.0f, back0 = truncf(0.5f * back);
+        const bool none = a_ref == -INFINITY && l == l;  // nothing seen, or only values of zero
+        const float norm0 = none ? 0.0f : ex2(back0), norm1 = none ? 0.0f : ex2(back - back0) / l;
         uint16_t *out = (uint16_t *)p.out + off;
         if (nt[t] > 0) {
             wait(&o_full[t], 0, KERR_MMA_WAIT);
@@ -1333,7 +1366,7 @@ attention_quant_long_kernel(const AttnQuant p, int skip_short, int span, uint32_
 #pragma unroll
                     for (int y = 0; y < 4; y++) {
                         // rows without positions: zeros (their columns of O may never have been written)
-                        const float a = len > 0 ? __uint_as_float(v[x + 2 * y]) * norm : 0.0f, b = len > 0 ? __uint_as_float(v[x + 2 * y + 1]) * norm : 0.0f;
+                        const float a = len > 0 ? __uint_as_float(v[x + 2 * y]) * norm0 * norm1 : 0.0f, b = len > 0 ? __uint_as_float(v[x + 2 * y + 1]) * norm0 * norm1 : 0.0f;
                         const __nv_bfloat162 z = __floats2bfloat162_rn(a, b);
                         h[y] = *reinterpret_cast<const uint32_t *>(&z);
                     }
@@ -1380,7 +1413,6 @@ attention_quant_long_kernel(const AttnQuant p, int skip_short, int span, uint32_
             asm volatile("cp.async.commit_group;" ::: "memory");
             page = page_of(j + 1);
         };
-        uint32_t power = 17u << 23;                      // R, which only grows
         if (n_tiles > 0) {
             page = page_of(0);
             ask(0);
@@ -1388,7 +1420,7 @@ attention_quant_long_kernel(const AttnQuant p, int skip_short, int span, uint32_
         for (int j = 0; j < n_tiles; j++) {
             const int b = j & 1, st = j % Sm::STAGES;
             const uint32_t there = there_next;
-            const bool ok = keys || scale_next <= 3.402823466e38f;       // a value's scale that is NaN or infinite: zeros, and marked
+            const bool ok = keys || fabsf(scale_next) <= 3.402823466e38f;       // a value's scale that is NaN or infinite: zeros, and marked
             const float scale = ok ? scale_next : 0.0f;
             auto publish = [&]() {
                 uint8_t *sc = lg_smem + Sm::SC + st * Sm::SCALES;
@@ -1402,24 +1434,29 @@ attention_quant_long_kernel(const AttnQuant p, int skip_short, int span, uint32_
                         fl.big[w] = big;
                     }
                 } else {
-                    float top = fmaxf(0.0f, scale);
+                    float top = fabsf(scale);
 #pragma unroll
                     for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
                     const uint32_t bad = __ballot_sync(0xffffffffu, !ok);
                     if (lane == 0) {
-                        top_s[b][w] = __float_as_uint(top);
+                        top_s[b][w] = top;
                         look_s[b][w] = there != 0xFFFFFFFFu || bad;      // positions past kv_end, on a page beyond the pool, or marked
                     }
                     __syncwarp();
                     named_barrier_sync(2, 128);          // what the four warps have found
-                    const uint32_t most = max(max(top_s[b][0], top_s[b][1]), max(top_s[b][2], top_s[b][3]));
-                    power = max(power, min((most + 0x7FFFFFu) & 0x7F800000u, 253u << 23));
+                    const uint32_t most = power_above(fmaxf(fmaxf(top_s[b][0], top_s[b][1]), fmaxf(top_s[b][2], top_s[b][3])));
+                    const uint32_t unit = min(most, 127u << 23);         // small values are made larger; larger ones would push others below
+                    const uint32_t wide = __ballot_sync(0xffffffffu, ok && (there >> lane & 1) && fabsf(scale) < __uint_as_float(most) * 0x1p-10f);
                     if (j >= Sm::STAGES) wait(&sc_empty[st], ((j / Sm::STAGES) & 1) ^ 1, KERR_EMPTY_WAIT);
-                    reinterpret_cast<float *>(sc + Sm::VW)[32 * w + lane] = scale * __uint_as_float((254u << 23) - power);
-                    if (lane == 0) fl.bad[w] = bad;
+                    reinterpret_cast<float *>(sc + Sm::VW)[32 * w + lane] = scale * __uint_as_float((254u << 23) - unit);
+                    if (lane == 0) {
+                        fl.bad[w] = bad;
+                        fl.wide[w] = wide;
+                    }
                     if (w == 0 && lane == 0) {
                         fl.all = !(look_s[b][0] | look_s[b][1] | look_s[b][2] | look_s[b][3]);
-                        fl.r_bits = power;
+                        fl.v_log = log2_of(most);
+                        fl.v_unit = log2_of(unit);
                     }
                 }
                 mbar_arrive(&sc_full[st]);

@@ -1036,6 +1036,11 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
         : "r"(taddr)
         : "memory");
 }
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0,%1,%2,%3,%4,%5,%6,%7};"
+                 ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(taddr)
+                 : "memory");
+}
 // Pairs of floats in one instruction.
 __device__ __forceinline__ float2 pair_op(float2 a, float2 b, float2 c) {
     float2 r;
@@ -1210,7 +1215,8 @@ attention_quant_long_kernel(const AttnQuant p, int skip_short, int span, uint32_
                 };
                 // Three forms of the code, chosen by the warp: most tiles are seen by every row whole, and a test a score costs
                 // more than the score's own arithmetic (MASKED); scales that differ by much are rare (WIDE).  Each 16 columns are
-                // asked for while the 16 before are worked on.
+                // asked for while the 16 before are worked on.  (Unrolled whole, or with weights stored 16 registers at a time,
+                // registers are spilled: 4096 tokens 252 us instead of 245.)
                 uint32_t v[2][16];
                 const float2 c2 = make_float2(c_row, c_row);
                 float mx = -INFINITY, mv = -INFINITY;    // of what the row sees: the largest score, at least the largest s + log2 vs
@@ -1219,38 +1225,42 @@ attention_quant_long_kernel(const AttnQuant p, int skip_short, int span, uint32_
                     float mx1 = -INFINITY, mv1 = -INFINITY;
                     tmem_ld16(s_col, v[0]);
                     tmem_ld_wait();
+#pragma unroll (MASKED ? 1 : 2)
+                    for (int cc = 0; cc < 4; cc++) {
 #pragma unroll
-                    for (int c = 0; c < 8; c++) {
-                        const uint32_t(&u)[16] = v[c & 1];
-                        tmem_ld16(s_col + 16 * ((c + 1) & 7), v[(c + 1) & 1]);           // after the last one the first again, for the weights
-                        uint32_t bits = 0;
-                        if constexpr (MASKED) bits = bits_of(c >> 1) >> (16 * (c & 1));
+                        for (int half = 0; half < 2; half++) {
+                            const int c = 2 * cc + half;
+                            const uint32_t(&u)[16] = v[half];
+                            tmem_ld16(s_col + 16 * ((c + 1) & 7), v[half ^ 1]);       // after the last one the first again, for the weights
+                            uint32_t bits = 0;
+                            if constexpr (MASKED) bits = bits_of(c >> 1) >> (16 * (c & 1));
 #pragma unroll
-                        for (int x = 0; x < 16; x += 4) {
-                            const float4 k4 = *reinterpret_cast<const float4 *>(ks + 16 * c + x);
-                            float2 ka = make_float2(k4.x, k4.y), kb = make_float2(k4.z, k4.w);
-                            if constexpr (WIDE) {        // a sum of codes and queries, below 2^30, times a scale of 2^98 would leave float32
-                                ka = pair_mul(ka, c2);
-                                kb = pair_mul(kb, c2);
+                            for (int x = 0; x < 16; x += 4) {
+                                const float4 k4 = *reinterpret_cast<const float4 *>(ks + 16 * c + x);
+                                float2 ka = make_float2(k4.x, k4.y), kb = make_float2(k4.z, k4.w);
+                                if constexpr (WIDE) {        // a sum of codes and queries, below 2^30, times a scale of 2^98 would leave float32
+                                    ka = pair_mul(ka, c2);
+                                    kb = pair_mul(kb, c2);
+                                }
+                                float2 a = pair_mul(make_float2(__uint_as_float(u[x]), __uint_as_float(u[x + 1])), ka);
+                                float2 d = pair_mul(make_float2(__uint_as_float(u[x + 2]), __uint_as_float(u[x + 3])), kb);
+                                if constexpr (MASKED) {
+                                    if (!(bits >> x & 1)) a.x = -INFINITY;
+                                    if (!(bits >> (x + 1) & 1)) a.y = -INFINITY;
+                                    if (!(bits >> (x + 2) & 1)) d.x = -INFINITY;
+                                    if (!(bits >> (x + 3) & 1)) d.y = -INFINITY;
+                                }
+                                if constexpr (WIDE) {
+                                    const float4 w4 = *reinterpret_cast<const float4 *>(vw + 16 * c + x);
+                                    auto share = [&](float score, float vs) { return vs == 0.0f ? -INFINITY : score + log2_of(power_above(fabsf(vs))); };
+                                    mv = fmaxf(mv, fmaxf(share(a.x, w4.x), share(a.y, w4.y)));
+                                    mv1 = fmaxf(mv1, fmaxf(share(d.x, w4.z), share(d.y, w4.w)));
+                                }
+                                mx = fmaxf(mx, fmaxf(a.x, a.y));
+                                mx1 = fmaxf(mx1, fmaxf(d.x, d.y));
                             }
-                            float2 a = pair_mul(make_float2(__uint_as_float(u[x]), __uint_as_float(u[x + 1])), ka);
-                            float2 d = pair_mul(make_float2(__uint_as_float(u[x + 2]), __uint_as_float(u[x + 3])), kb);
-                            if constexpr (MASKED) {
-                                if (!(bits >> x & 1)) a.x = -INFINITY;
-                                if (!(bits >> (x + 1) & 1)) a.y = -INFINITY;
-                                if (!(bits >> (x + 2) & 1)) d.x = -INFINITY;
-                                if (!(bits >> (x + 3) & 1)) d.y = -INFINITY;
-                            }
-                            if constexpr (WIDE) {
-                                const float4 w4 = *reinterpret_cast<const float4 *>(vw + 16 * c + x);
-                                auto share = [&](float score, float vs) { return vs == 0.0f ? -INFINITY : score + log2_of(power_above(fabsf(vs))); };
-                                mv = fmaxf(mv, fmaxf(share(a.x, w4.x), share(a.y, w4.y)));
-                                mv1 = fmaxf(mv1, fmaxf(share(d.x, w4.z), share(d.y, w4.w)));
-                            }
-                            mx = fmaxf(mx, fmaxf(a.x, a.y));
-                            mx1 = fmaxf(mx1, fmaxf(d.x, d.y));
+                            tmem_ld_wait();
                         }
-                        tmem_ld_wait();
                     }
                     mx = fmaxf(mx, mx1);
                     if constexpr (!WIDE) mx *= c_row;
@@ -1286,47 +1296,51 @@ attention_quant_long_kernel(const AttnQuant p, int skip_short, int span, uint32_
                     const float2 nb = make_float2(-from, -from);
                     float2 l2 = make_float2(0.0f, 0.0f);
                     bool bad = false;
-                    uint32_t w[16];
+                    uint32_t w[8];
+#pragma unroll (MASKED ? 1 : 2)
+                    for (int cc = 0; cc < 4; cc++) {
 #pragma unroll
-                    for (int c = 0; c < 8; c++) {
-                        const uint32_t(&u)[16] = v[c & 1];
-                        if (c < 7) tmem_ld16(s_col + 16 * (c + 1), v[(c + 1) & 1]);
-                        uint32_t bits = 0;
-                        if constexpr (MASKED) {
-                            bits = bits_of(c >> 1);
-                            bad |= (bits & fl.bad[c >> 1]) != 0;
-                            bits >>= 16 * (c & 1);
-                        }
-#pragma unroll
-                        for (int x = 0; x < 16; x += 4) {
-                            const float4 k4 = *reinterpret_cast<const float4 *>(ks + 16 * c + x), w4 = *reinterpret_cast<const float4 *>(vw + 16 * c + x);
-#pragma unroll
-                            for (int y = 0; y < 2; y++) {
-                                const int at = x + 2 * y;
-                                const float2 s2 = make_float2(__uint_as_float(u[at]), __uint_as_float(u[at + 1]));
-                                const float2 k2 = y ? make_float2(k4.z, k4.w) : make_float2(k4.x, k4.y), v2 = y ? make_float2(w4.z, w4.w) : make_float2(w4.x, w4.y);
-                                float2 e, z;             // what the sum gets, the weights
-                                if constexpr (APART) {
-                                    const float2 score = pair_mul(s2, pair_mul(k2, c2));
-                                    e = make_float2(ex2(score.x - m_base), ex2(score.y - m_base));
-                                    const uint32_t px = power_of(fabsf(v2.x)), py = power_of(fabsf(v2.y));       // vs = 2^p times its rest
-                                    z.x = ex2((score.x - from) + log2_of(px)) * (v2.x * __uint_as_float((254u << 23) - px));
-                                    z.y = ex2((score.y - from) + log2_of(py)) * (v2.y * __uint_as_float((254u << 23) - py));
-                                } else {
-                                    e = pair_op(pair_mul(s2, k2), c2, nb);
-                                    e = make_float2(ex2(e.x), ex2(e.y));
-                                }
-                                if constexpr (MASKED) {
-                                    if (!(bits >> at & 1)) e.x = z.x = 0.0f;
-                                    if (!(bits >> (at + 1) & 1)) e.y = z.y = 0.0f;
-                                }
-                                l2 = pair_add(l2, e);
-                                if constexpr (!APART) z = pair_mul(e, v2);
-                                w[8 * (c & 1) + at / 2] = pack_f16(z.x, z.y);
+                        for (int half = 0; half < 2; half++) {
+                            const int c = 2 * cc + half;
+                            const uint32_t(&u)[16] = v[half];
+                            if (c < 7) tmem_ld16(s_col + 16 * (c + 1), v[half ^ 1]);
+                            uint32_t bits = 0;
+                            if constexpr (MASKED) {
+                                bits = bits_of(c >> 1);
+                                bad |= (bits & fl.bad[c >> 1]) != 0;
+                                bits >>= 16 * (c & 1);
                             }
+#pragma unroll
+                            for (int x = 0; x < 16; x += 4) {
+                                const float4 k4 = *reinterpret_cast<const float4 *>(ks + 16 * c + x), w4 = *reinterpret_cast<const float4 *>(vw + 16 * c + x);
+#pragma unroll
+                                for (int y = 0; y < 2; y++) {
+                                    const int at = x + 2 * y;
+                                    const float2 s2 = make_float2(__uint_as_float(u[at]), __uint_as_float(u[at + 1]));
+                                    const float2 k2 = y ? make_float2(k4.z, k4.w) : make_float2(k4.x, k4.y), v2 = y ? make_float2(w4.z, w4.w) : make_float2(w4.x, w4.y);
+                                    float2 e, z;             // what the sum gets, the weights
+                                    if constexpr (APART) {
+                                        const float2 score = pair_mul(s2, pair_mul(k2, c2));
+                                        e = make_float2(ex2(score.x - m_base), ex2(score.y - m_base));
+                                        const uint32_t px = power_of(fabsf(v2.x)), py = power_of(fabsf(v2.y));       // vs = 2^p times its rest
+                                        z.x = ex2((score.x - from) + log2_of(px)) * (v2.x * __uint_as_float((254u << 23) - px));
+                                        z.y = ex2((score.y - from) + log2_of(py)) * (v2.y * __uint_as_float((254u << 23) - py));
+                                    } else {
+                                        e = pair_op(pair_mul(s2, k2), c2, nb);
+                                        e = make_float2(ex2(e.x), ex2(e.y));
+                                    }
+                                    if constexpr (MASKED) {
+                                        if (!(bits >> at & 1)) e.x = z.x = 0.0f;
+                                        if (!(bits >> (at + 1) & 1)) e.y = z.y = 0.0f;
+                                    }
+                                    l2 = pair_add(l2, e);
+                                    if constexpr (!APART) z = pair_mul(e, v2);
+                                    w[at / 2] = pack_f16(z.x, z.y);
+                                }
+                            }
+                            if (c < 7) tmem_ld_wait();
+                            tmem_st8(s_col + 8 * c, w);
                         }
-                        if (c < 7) tmem_ld_wait();
-                        if (c & 1) tmem_st16(s_col + 16 * (c >> 1), w);
                     }
                     l += APART ? l2.x + l2.y : (l2.x + l2.y) * ex2(from - m_base);
                     if (MASKED && bad) l = __int_as_float(0x7FC00000);   // sees a value that is NaN

@@ -289,7 +289,7 @@ int llmrs_cuda_embed(llmrs_ctx *ctx, llmrs_buf *out, const llmrs_buf *table, con
  *
  * Index buffers are device memory: what they name is checked by the kernels.  A slot, page or length beyond
  * the pool or the page table is neither read nor written, and the next llmrs_cuda_sync / read_f32 returns
- * LLMRS_ERR_ARG.  All buffers must live on the context's device, and outputs must not overlap inputs except
+ * LLMRS_ERR_ARG.  At most 2^30 - 1 tokens, heads of a token and requests in a call.  All buffers must live on the context's device, and outputs must not overlap inputs except
  * where a call says so. */
 
 /* How rope frequencies are stretched for a context of more positions than the model was trained on. */

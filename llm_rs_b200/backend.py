@@ -195,7 +195,7 @@ def rope_frequencies(rotary_dim: int, rope_theta: float, kind: RopeScaling = Rop
     take: rope_theta^(-2 i / rotary_dim), stretched as `kind` says, divided by `factors` (a file's rope_freqs.weight).
     `low` and `high` are turns over the original context: usually 1 and 4 for WAVELENGTH, 1 and 32 for YARN.  No GPU."""
     lib = load_library()
-    if rotary_dim < 0 or original_context < 0:
+    if not (0 <= rotary_dim < 1 << 32 and 0 <= original_context < 1 << 32):
         raise ValueError(f"rope_frequencies: rotary_dim {rotary_dim}, original_context {original_context}")
     out = np.empty(max(rotary_dim // 2, 1), dtype=np.float32)
     mag = C.c_float()

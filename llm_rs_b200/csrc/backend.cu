@@ -1083,6 +1083,7 @@ int llmrs_cuda_attention(llmrs_ctx *ctx, llmrs_buf *out, const llmrs_buf *q, con
 // ---- scaled rotary positions and the 8-bit KV cache ------------------------------------------------
 
 static uint32_t buf_cols(const llmrs_buf *b) { return b->dim1 ? b->dim1 : 1; }
+constexpr uint64_t QUANT_MOST = 0x3FFFFFFF;    // tokens, heads of a token, requests: the kernels count them, and a grid's share more, in ints
 static bool bufs_overlap(const llmrs_buf *a, const llmrs_buf *b) {
     const uintptr_t pa = (uintptr_t)a->dptr, pb = (uintptr_t)b->dptr;
     return pa < pb + b->nbytes && pb < pa + a->nbytes;
@@ -1161,7 +1162,8 @@ static int rope_table_ok(llmrs_ctx *ctx, const char *name, const llmrs_buf *q, c
     if (!dense_elem_bytes(q->dtype) || k->dtype != q->dtype || positions->dtype != LLMRS_I32 || inv_freq->dtype != LLMRS_F32)
         return ctx->fail(LLMRS_ERR_DTYPE, "%s: activations of one type (F32 or BF16), positions I32, inv_freq F32", name);
     if (head_dim == 0 || head_dim % 2 || head_dim > 256 || q->dim0 % head_dim || k->dim0 % head_dim || buf_cols(k) != buf_cols(q) ||
-        buf_elems(positions) < buf_cols(q) || inv_freq->dim1 > 1 || inv_freq->dim0 > head_dim / 2)
+        buf_elems(positions) < buf_cols(q) || inv_freq->dim1 > 1 || inv_freq->dim0 > head_dim / 2 || buf_cols(q) > QUANT_MOST ||
+        ((uint64_t)q->dim0 + 2ull * k->dim0) / head_dim > QUANT_MOST)
         return ctx->fail(LLMRS_ERR_SHAPE, "%s: q [%u, %u], k [%u, %u], head_dim %u, %zu positions, inv_freq [%u]", name, q->dim0, q->dim1,
                          k->dim0, k->dim1, head_dim, buf_elems(positions), inv_freq->dim0);
     if (!std::isfinite(magnitude)) return ctx->fail(LLMRS_ERR_ARG, "%s: magnitude is not finite", name);
@@ -1205,7 +1207,8 @@ int llmrs_cuda_scatter_kv_quant(llmrs_ctx *ctx, llmrs_buf *pool, llmrs_buf *scal
     if (int rc = quant_pool_ok(ctx, name, pool, scales)) return rc;
     if (!dense_elem_bytes(src->dtype) || slot_mapping->dtype != LLMRS_I32)
         return ctx->fail(LLMRS_ERR_DTYPE, "%s: src F32 or BF16, slot_mapping I32", name);
-    if (src->dim0 != pool->dim0 || num_tokens > buf_cols(src) || num_tokens > buf_elems(slot_mapping))
+    if (src->dim0 != pool->dim0 || num_tokens > buf_cols(src) || num_tokens > buf_elems(slot_mapping) || num_tokens > QUANT_MOST ||
+        buf_cols(scales) > QUANT_MOST)
         return ctx->fail(LLMRS_ERR_SHAPE, "%s: %u tokens of src [%u, %u] into rows of %u, %zu slots", name, num_tokens, src->dim0,
                          src->dim1, pool->dim0, buf_elems(slot_mapping));
     if (int rc = quant_overlap_ok(ctx, name, all, 4, 0)) return rc;
@@ -1318,7 +1321,7 @@ int llmrs_cuda_attention_quant(llmrs_ctx *ctx, llmrs_buf *out, const llmrs_buf *
                          v_scales->dim1, n_kv_heads, head_dim);
     const uint64_t total_q = buf_elems(q) / row, num_req = buf_elems(seq_lens);
     if (buf_elems(q) % row || buf_elems(out) != buf_elems(q) || buf_elems(query_starts) < num_req + 1 ||
-        buf_elems(block_table) / max_blocks_per_seq < num_req || total_q * n_heads > 0x7FFFFFFFull)
+        buf_elems(block_table) / max_blocks_per_seq < num_req || total_q * n_heads > 0x7FFFFFFFull || num_req > QUANT_MOST)
         return ctx->fail(LLMRS_ERR_SHAPE, "%s: q of %zu values, %zu requests, %zu query_starts, %zu page entries", name, buf_elems(q),
                          (size_t)num_req, buf_elems(query_starts), buf_elems(block_table));
     if (int rc = quant_overlap_ok(ctx, name, all, 9, 0)) return rc;

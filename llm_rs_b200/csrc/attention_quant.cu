@@ -370,9 +370,6 @@ template <int RB, int TP> struct Walk {
     }
 };
 
-// The consumer threads of a CTA: joins n parts of HW heads x n_rows rows, into the output (`last`) or into the first of
-// their slots.  Four elements (16 bytes) of the result a thread and two parts of each at a time, with their maxima and
-// sums: 16 loads under way (four parts at a time: 112 us instead of 108 for 64 ragged requests).
 // Loads that stay where they are, in front of what uses them, and come from L2 (other CTAs have just written there).
 __device__ __forceinline__ float4 load_part4(const float *p) {
     float4 v;
@@ -398,6 +395,9 @@ struct Join {
     int n, slot0, step, slot1;                           // part 0 is in slot slot0, part i > 0 in slot1 + (i - 1) * step
     bool last;
 };
+// The consumer threads of a CTA: joins n parts of HW heads x n_rows rows, into the output (`last`) or into the first of
+// their slots.  Four elements (16 bytes) of the result a thread and two parts of each at a time, with their maxima and
+// sums: 16 loads under way (four parts at a time: 112 us instead of 108 for 64 ragged requests).
 template <int HD, int RB, int HW>
 __device__ __noinline__ void join_parts(const Join &j) {     // not inlined: its registers are not the main loop's
     constexpr int E = 4, B = 2;
@@ -1011,7 +1011,7 @@ struct LongFlags {                   // of a tile of positions, 32 to a warp
     float v_log, v_unit;             // log2 of a power of two that no value's scale exceeds, and of the unit of those in VW
 };
 template <int HD> struct LongSmem {
-    static constexpr int HALVES = HD / 64, TILE = LG_ROWS * HD * 2;      // 128 rows of f16, in halves of 64 dimensions
+    static constexpr int TILE = LG_ROWS * HD * 2;        // 128 rows of f16, in halves of 64 dimensions
     static constexpr int Q = 0, K = 2 * TILE, V = K + 2 * TILE, RAW = V + 2 * TILE, SC = RAW + 2 * (TILE / 2);
     static constexpr int STAGES = 2, KS = 0, VW = 512, SCALES = 1024;    // of a tile of positions: ks [128], vs / 2^v_unit [128]
     static constexpr int BYTES = SC + STAGES * SCALES;

@@ -1288,7 +1288,7 @@ int llmrs_cuda_gather_quant(llmrs_ctx *ctx, llmrs_buf *out, const llmrs_buf *poo
     if (e == cudaSuccess)
         e = launch_gather_quant(out->dptr, (int)out->dtype, (const uint8_t *)pool->dptr, (const float *)scales->dptr,
                                 (const uint32_t *)indices->dptr, pool->dim0, pool->dim0 / buf_cols(scales), buf_cols(pool),
-                                num_indices, ctx->dev_error, ctx->stream, ctx->pdl);
+                                num_indices, ctx->dev_error, ctx->sm_count, ctx->stream, ctx->pdl);
     if (e != cudaSuccess) return ctx->cuda_fail(e, name);
     ctx->launches++;
     return LLMRS_OK;

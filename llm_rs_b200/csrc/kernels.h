@@ -109,7 +109,6 @@ cudaError_t launch_attention(const void *q, const void *k_pool, const void *v_po
                              int block_size, int max_blocks_per_seq, cudaStream_t s, bool pdl);
 
 // ---- scaled rotary positions and the 8-bit KV cache (kv_quant.cu, attention_quant.cu) ----
-constexpr int DT_E4M3 = 256;         // codes of the 8-bit cache; not a GGUF type
 // One pass over the rows of `tokens` tokens: q and k rotated by the table inv_freq [rotary / 2] and scaled
 // by `magnitude`, q to q_out, k to k_out or (k_pool) quantised into its slot, v quantised into its slot.
 // nq, nk, nv: heads of each (0: not there).  slots null: no cache.  head_dim even, at most 256.
@@ -130,7 +129,7 @@ cudaError_t launch_rope_write(const RopeWrite &p, int dtype, int tokens, int sm_
 // out[c] (F32 or BF16) = codes * scales of slot indices[c], c < rows.
 cudaError_t launch_gather_quant(void *out, int dtype, const uint8_t *pool, const float *scales, const uint32_t *indices,
                                 uint32_t kv_dim, uint32_t head_dim, uint32_t num_slots, uint32_t rows, uint32_t *err,
-                                cudaStream_t s, bool pdl);
+                                int sm_count, cudaStream_t s, bool pdl);
 // Paged attention over the 8-bit cache; the arguments of llmrs_cuda_attention_quant.
 struct AttnQuant {
     const void *q;

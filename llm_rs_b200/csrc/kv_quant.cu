@@ -331,14 +331,14 @@ cudaError_t launch_rope_write(const RopeWrite &p, int dtype, int tokens, int sm_
 
 cudaError_t launch_gather_quant(void *out, int dtype, const uint8_t *pool, const float *scales, const uint32_t *indices,
                                 uint32_t kv_dim, uint32_t head_dim, uint32_t num_slots, uint32_t rows, uint32_t *err,
-                                cudaStream_t s, bool pdl) {
+                                int sm_count, cudaStream_t s, bool pdl) {
     if (rows == 0) return cudaSuccess;
     const uint32_t vec = dtype == DT_BF16 ? 16 : 8;      // 32 bytes of output
     const bool ok = head_dim % vec == 0 && (uintptr_t)out % 32 == 0;
     const size_t n = (size_t)(kv_dim / (ok ? vec : 1)) * rows;
     constexpr int N = 4;
     // four units a thread once that still leaves every SM its share of warps; one each below
-    const int per = n >= (size_t)4 * 256 * 148 * 4 ? N : 1;
+    const int per = n >= (size_t)4 * 256 * sm_count * 4 ? N : 1;
     const dim3 grid((unsigned)((n + 256 * per - 1) / (256 * per)));
 #define LLMRS_GATHER(T, V, K) launch_dependent(gather_quant_kernel<T, V, K>, grid, dim3(256), 0, s, pdl, (T *)out, pool, scales, \
                                                indices, kv_dim, head_dim, num_slots, rows, err)

@@ -1168,7 +1168,6 @@ attention_quant_long_kernel(const AttnQuant p, int skip_short, int span, uint32_
         const bool on = t * LG_ROWS + i < rows;
         const int len = on ? r.before + rr / group + 1 : 0;
         const int min_len = r.before + (row0 + t * LG_ROWS) / group + 1;         // what the tile's first row sees
-        const bool full_tile = rows >= (t + 1) * LG_ROWS;
         const size_t off = on ? ((size_t)(r.first + rr / group) * p.n_heads + (size_t)kvh * group + rr % group) * HD : 0;
         // the row of queries: its size, then scaled by a power of two to f16 and into the operand's layout
         float amax = 0.0f;
@@ -1205,7 +1204,7 @@ attention_quant_long_kernel(const AttnQuant p, int skip_short, int span, uint32_
                 const float *ks = reinterpret_cast<const float *>(sc + Sm::KS), *vw = reinterpret_cast<const float *>(sc + Sm::VW);
                 const LongFlags &fl = flags_s[st];
                 const bool wide = (fl.wide[0] | fl.wide[1] | fl.wide[2] | fl.wide[3] | fl.big[0] | fl.big[1] | fl.big[2] | fl.big[3]) != 0;
-                const bool masked = !full_tile || (j + 1) * LG_POS > min_len || fl.all == 0 || wide;
+                const bool masked = (j + 1) * LG_POS > min_len || fl.all == 0 || wide;     // (rows past the end do what the others do, for nothing)
                 wait(&s_full[t], j & 1, KERR_MMA_WAIT);
                 tc_fence_after();
                 auto bits_of = [&](int c) -> uint32_t {  // which of the 32 positions of chunk c this row sees

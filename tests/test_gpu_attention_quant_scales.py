@@ -155,6 +155,26 @@ def test_keys_of_all_sizes(backend, hd, news):
         check(out, *wanted(q, kc, ks, vc, vs, slots[0], news, nh, nkv, hd), l, torch.bfloat16)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("hd,news", [(64, 1), (128, 4), (64, 70), (128, 150), (96, 2)])
+def test_scales_of_either_sign_and_of_zero(backend, hd, news, dtype):
+    """A cache that something else has filled: a third of the scales negative, a fifth zero; one head's values all zero, which
+    makes its rows zero; one head's below float32's normal range but for one."""
+    nh, nkv, block, l = 8, 4, 16, 300
+    kc, ks, vc, vs, table, slots, most = paged_cache(nkv, hd, [l], block, 470)
+    g = torch.Generator().manual_seed(471)
+    for s in (ks, vs):
+        pick = torch.rand(nkv, l, generator=g)
+        s[:, slots[0]] *= torch.where(pick < 1 / 3, -1.0, torch.where(pick < 1 / 3 + 1 / 5, 0.0, 1.0)).cuda()
+    vs[2, slots[0]] = 0.0
+    vs[3, slots[0]] = 2.0 ** -130
+    vs[3, slots[0][7]] = 2.0 ** -100
+    q = rand(news, nh * hd, seed=472, loud=False).to(dtype)
+    out = attend(backend, q, kc, ks, vc, vs, table, [l], [news], nh, nkv, hd, block, most)
+    check(out, *wanted(q, kc, ks, vc, vs, slots[0], news, nh, nkv, hd), l, dtype)
+    assert not out.view(news, nkv, -1)[:, 2].any()
+
+
 @pytest.mark.parametrize("group,tokens", [(1, 65), (3, 11), (4, 33), (5, 27), (7, 19), (8, 17), (17, 5), (32, 1)])
 @pytest.mark.parametrize("hd", [64, 128])
 def test_row_counts_that_end_inside_a_warp(backend, hd, group, tokens):

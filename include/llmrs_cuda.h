@@ -285,7 +285,12 @@ int llmrs_cuda_embed(llmrs_ctx *ctx, llmrs_buf *out, const llmrs_buf *table, con
  * code = E4M3(value / scale), rounded to nearest even: half a step of E4M3, 2^-4 of a value, at most, or 2^-10
  * scale of one below 2^-6 scale.  A head with a value that is not finite gets the scale NaN and codes 0: rows of
  * attention that see the position come out NaN, others do not notice.  The pools need no initialisation; codes
- * other than those the write calls make must be finite (not 0x7F / 0xFF).
+ * other than those the write calls make must be finite (not 0x7F / 0xFF); scales may be
+ * of either sign, up to 2^126, and NaN or infinite, which is NaN to the rows that see it.
+ *
+ * Any even head_dim up to 256 is taken.  Wide accesses need head_dim a multiple of 16 (BF16) or 8 (F32), for split_half also
+ * rotary_dim / 2 a multiple of half as many, and for gather_quant `out` on 32 bytes; without, values go one by one, several
+ * times slower.
  *
  * Index buffers are device memory: what they name is checked by the kernels.  A slot, page or length beyond
  * the pool or the page table is neither read nor written, and the next llmrs_cuda_sync / read_f32 returns
@@ -351,7 +356,10 @@ int llmrs_cuda_gather_quant(llmrs_ctx *ctx, llmrs_buf *out, const llmrs_buf *poo
  * its arguments of the same meaning.  q and out F32 or BF16, of one type; n_heads any multiple of n_kv_heads,
  * head_dim a multiple of 32, at most 256.  Positions on a page beyond the pool count as unseen; a query token that
  * sees no position (its request is shorter than its query tokens) yields zeros; tokens behind the last
- * request keep what out held.  Like llmrs_cuda_attention it uses a workspace of the context, so graphs captured
+ * request keep what out held.  A row depends on the positions that it sees and on nothing else.  Codes and BF16 queries enter the
+ * matrix products exactly, scales and sums are float32; a weight is rounded to f16 (2^-11 of it; F32: to two of them), counted from
+ * the row's largest share.  Made for head_dim 64 and 128; others are right, but slower by two orders of magnitude.  More than
+ * 16 rows (query tokens x n_heads / n_kv_heads) of a request are worked on by one SM for 128 or 256 rows, whatever its length.  Like llmrs_cuda_attention it uses a workspace of the context, so graphs captured
  * from one context must not run at the same time. */
 int llmrs_cuda_attention_quant(llmrs_ctx *ctx, llmrs_buf *out, const llmrs_buf *q, const llmrs_buf *k_pool,
                                const llmrs_buf *k_scales, const llmrs_buf *v_pool, const llmrs_buf *v_scales,

@@ -160,7 +160,7 @@ __global__ void __launch_bounds__(AQ_TILE) attention_quant_simple_kernel(const A
 // each 18 neighbours joins theirs, and the last of those the rest, always in the order of the parts (few requests:
 // attention_quant_merge_kernel).
 //
-// One request of 131071 positions: 57 us, 74 % of the measured HBM rate; without the joining 49 (86 %).  64 requests of
+// One request of 131071 positions: 56 us, 76 % of the measured HBM rate; without the joining 48 (88 %).  64 requests of
 // 100 to 8192: 108 us, 79 %; without 97 (88 %).
 //
 // A CTA has 4 consumer warps, HW heads x PW times 32 positions, so that neighbouring heads of a slot, neighbours
@@ -974,7 +974,7 @@ attention_quant_short_kernel(const __grid_constant__ ShortMaps maps, const AttnQ
 }
 
 // ---- many rows: prompts and chunks of prompts -------------------------------------------------------
-// Bound by the tensor cores (tcgen05, f16 operands, float32 accumulators in TMEM), then by the exponentials: a score costs
+// The floor is the tensor cores' (tcgen05, f16 operands, float32 accumulators in TMEM), then the exponentials': a score costs
 // 4 head_dim operations, 512 of a tensor core's cycles for 128 x 128 of them, and one ex2, 1024 cycles of the
 // SM's 16 a cycle.  So a CTA keeps two tiles of 128 query rows (token x head of the group, packed) against one
 // stream of keys and values: while one tile's weights are formed the tensor cores work for the other.
@@ -987,7 +987,7 @@ attention_quant_short_kernel(const __grid_constant__ ShortMaps maps, const AttnQ
 //                    as they come, positions in rows, so they are the operand's major dimension the other way round).
 //
 // Softmax in one pass.  The sum refers to a maximum m of the row's scores and O to a of its s + log2 vs, both only moved when
-// outgrown by more than 6 (log2), so O is rarely rescaled (2 instead of 6: 4096 tokens 207 us instead of 191, at that step).
+// outgrown by more than 6 (log2), so O is rarely rescaled (2 instead of 6: 4096 tokens 251 us instead of 244).
 // Weights enter as e^s vs / 2^a * 2^9, below 2^15: f16 keeps 2^-11 of a weight.
 //
 // The codes, exact in f16, are what is multiplied; ks enters at the score and vs at the weight, in float32.  Multiplied
@@ -996,9 +996,14 @@ attention_quant_short_kernel(const __grid_constant__ ShortMaps maps, const AttnQ
 // is off by a tenth.
 //
 // Only what a row sees decides its references.  In a tile of positions whose vs lie within 2^10 of one another the row's largest
-// score plus log2 of the tile's largest vs does for a, at most 10 too much, so f16 keeps a weight down to 2^-24 of the largest; in
-// others a is found position by position, and a weight has an exponential of its own.  A value whose scale is not finite is zero
-// there, and the rows that see it are marked, so that no row sees NaN times zero.
+// score plus log2 of the tile's largest vs does for a, at most 10 too much: f16 keeps all bits of a weight down to 2^-13 of the
+// largest, and 2^-24 of the largest below; in other tiles a is found position by position, and a weight has an exponential of
+// its own.  A value whose scale is not finite is zero there, and the rows that see it are marked, so that no row sees NaN
+// times zero.
+//
+// 4096 tokens of 32 heads over 8: 244 us, 0.56 PFLOP/s (33 % of the measured rate); 1152 tokens behind 31616: 0.69 (41 %).  There a
+// chain of waits bounds it, not one unit: tensor pipe 25 % busy, issue slots 41 %, exponentials 28 %, the shared memory's
+// pipe 58 % (a quarter of it bank conflicts of the converting warps), eight warps with weights waiting for TMEM and for scales.
 constexpr int LG_ROWS = 128, LG_POS = 128, LG_THREADS = 17 * 32;
 constexpr float LG_SLACK = 6.0f;     // log2: the weights' factor 2^9 leaves these octaves to f16's 65504
 
@@ -1560,8 +1565,8 @@ attention_quant_long_kernel(const AttnQuant p, int skip_short, int span, uint32_
 template <int HD>
 cudaError_t launch_long(const AttnQuant &p, int skip_short, int sm_count, uint32_t polls, cudaStream_t s, bool pdl) {
     // 256 rows a CTA, so that two tiles share keys and values and hide each other's waits; one tile of 128 where that is about
-    // a CTA an SM or less (1.25: requests differ in length).  128 tokens of 32 heads over 8: 11.9 us with one tile, 16.4 with
-    // two; 128 behind 8064: 140 and 160; 12 chunks of up to 500 tokens, 2 KV heads: 76 and 88; but 1152 tokens: 40.5 and 36.6.
+    // a CTA an SM or less (1.25: requests differ in length).  128 tokens of 32 heads over 8: 12.2 us with one tile, 17.0 with
+    // two; 128 behind 8064: 187 and 227; 12 chunks of up to 500 tokens, 2 KV heads: 78 and 93; but 1152 tokens: 45.9 and 44.0.
     const long long rows = (long long)p.total_q * (p.n_heads / p.n_kv);
     const int span = rows * p.n_kv <= (long long)sm_count * LG_ROWS * 5 / 4 ? LG_ROWS : 2 * LG_ROWS;
     // every request may end in a block that is not full; the short kernel's, of at most SHORT_ROWS rows, have none
@@ -1579,7 +1584,7 @@ ShortPlan short_plan(const AttnQuant &p, int dtype) {
     const int group = p.n_heads / p.n_kv;
     ShortPlan s;
     // Rows per block: 16 rows cost little more than 8, but a block of 8 leaves registers for nothing to be spilled (64 decode
-    // requests: 108 us against 123).  So 8 where that holds what a request has on average, and in batches that mix prompts,
+    // requests: 107 us against 131).  So 8 where that holds what a request has on average, and in batches that mix prompts,
     // the long kernel's, with single tokens; 16 for drafts of a few tokens, and for F32 prompts.
     const double rows = (double)p.total_q * group / p.num_req;
     s.rb = group <= 8 && (rows <= 8 || (rows > SHORT_ROWS && dtype == DT_BF16)) ? 8 : 16;
@@ -1654,8 +1659,8 @@ cudaError_t launch_short_hw(const AttnQuant &p, int hw, const ShortCall &c) {
     }
 }
 // The parts of one row (query token, head), joined in order: the form for few requests, each in many parts, where a CTA a
-// row has more loads under way than the CTAs that happen to be last (one request of 131071 positions, 148 parts a row: 57 us
-// in all instead of 67, one of 1000: 11.9 instead of 14.4).  Looking its request up costs a CTA too much where there are many
+// row has more loads under way than the CTAs that happen to be last (one request of 131071 positions, 148 parts a row: 56 us
+// in all instead of 66, one of 1000: 12.7 instead of 15.2).  Looking its request up costs a CTA too much where there are many
 // (64 requests: 65 us for this kernel beside 97), and there are few parts a row to join then.
 template <int HD>
 __global__ void __launch_bounds__(MERGE_THREADS)

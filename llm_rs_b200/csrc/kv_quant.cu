@@ -114,8 +114,8 @@ __device__ __forceinline__ void rotate(float &a, float &b, float2 t) {
 // position 131072 a float32 angle has lost 7 of its fraction's bits) and shared by its 40 or so heads.
 // HBM-bound: what is read and written is what the operation cannot do without.  So a thread asks for the units of
 // PRE rows before anything else; the angles are formed while they are under way.  8192 tokens, 32 + 8 heads of 128, bf16:
-// rotated 30.9 us (5.4 TB/s, 83 % of the measured rate); rotated and written 43.4 (65 %), there bound by issue slots, the
-// rows that are quantised taking twice the instructions of the others.
+// rotated 31 us (5.4 TB/s, 82 % of the measured rate); rotated and written 43.4 (65 %), where 28 M warp instructions take 63 %
+// of the issue slots, the cosines' reads, half of them bank conflicts, keep L1's pipe 71 % busy, and 25 warps an SM do not hide both.
 template <typename T, int V, int ITER, int PRE, bool HALF>
 __global__ void __launch_bounds__(RW_THREADS, ITER == 1 ? 7 : 1) rope_write_kernel(const RopeWrite p) {
     using C = Chunk<T, V>;

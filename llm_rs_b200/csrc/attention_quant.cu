@@ -1020,6 +1020,7 @@ template <int HD> struct LongSmem {
     static constexpr int Q = 0, K = 2 * TILE, V = K + 2 * TILE, RAW = V + 2 * TILE, SC = RAW + 2 * (TILE / 2);
     static constexpr int STAGES = 2, KS = 0, VW = 512, SCALES = 1024;    // of a tile of positions: ks [128], vs / 2^v_unit [128]
     static constexpr int BYTES = SC + STAGES * SCALES;
+    static_assert(BYTES + 1024 <= 227 * 1024, "with the static shared memory, which starts the dynamic part on 1024 bytes");
 };
 
 __device__ __forceinline__ void umma_f16_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
